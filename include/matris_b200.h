@@ -405,6 +405,104 @@ int mb_layernorm_bwd(int64_t n_rows, const float* x, const float* w, const float
 int mb_rmsnorm_fwd(int64_t n_rows, const float* x, const float* w, float* y, void* stream);
 int mb_rmsnorm_bwd(int64_t n_rows, const float* x, const float* w, const float* dy, float* dx, void* stream);
 
+/* ------------------------------------------------------------------ row types of the norm and the router */
+#define MB_DTYPE_F32 0
+#define MB_DTYPE_BF16 1
+#define MB_DTYPE_F16 2
+
+/* Group norm with an optional SiLU over the rows of every structure, features last.  Statistics of a (segment, group) go over the
+ * segment's rows and the group's channels / groups channels, in float32:
+ *   xh = (x - mean) rstd, z = xh weight + bias, y = z or SiLU(z).
+ * Segment s is rows seg_ptr[s] .. seg_ptr[s+1] - 1; seg_ptr NULL: n_seg segments of n_rows / n_seg rows.  Offsets outside
+ * [0, n_rows] are cut to it.  Rows of no segment are left as they are, or set to zero with zero_rest.  weight or bias NULL: 1, 0.
+ * channels <= 1024, any row alignment (rows of 16-byte pieces take wide accesses); n_rows < 2^31.
+ * bwd reads stats and writes dx and, where given, dweight and dbias [channels] (sums over all segments, in a fixed order).
+ * scratch: mb_group_norm_scratch() bytes, 16-byte aligned, free again when the call's work is done. */
+typedef struct mb_group_norm {
+  int64_t n_rows;
+  int32_t n_seg, channels, groups, dtype, act, zero_rest; /* dtype of x, y, dy, dx; act: 0 none, 1 SiLU */
+  float eps; int32_t pad0;
+  const int32_t* seg_ptr;
+  const void* x; int64_t ld_x;
+  const float* weight; const float* bias;
+  void* y; int64_t ld_y;
+  float* stats;                                           /* [n_seg, groups, 2]: mean, rstd; written by fwd, read by bwd */
+  const void* dy; int64_t ld_dy;
+  void* dx; int64_t ld_dx;
+  float* dweight; float* dbias;
+  void* scratch;
+} mb_group_norm;
+size_t mb_group_norm_scratch(int64_t n_rows, int32_t n_seg, int32_t channels);
+int mb_group_norm_fwd(const mb_group_norm* d, void* stream);
+int mb_group_norm_bwd(const mb_group_norm* d, void* stream);
+
+/* ------------------------------------------------------------------ mixture of experts
+ * Router: p = softmax(logits) over a row's available experts (logit > -inf), the top_k largest (equal ones: the lowest index first),
+ * weights p, or p over their sum with renorm.  A row with valid[r] = 0 or without an available expert is not routed: ids -1, weights 0.
+ * Where fewer than top_k are available the rest of the row is filled the same way.
+ *   counts[e] = rows that take e, counts[n_experts] = T = rows routed, loss = n_experts / (top_k T^2) sum_e counts[e] sum_r p[r,e]
+ *   (0 for T = 0; 1 when both are even)
+ * Grouping: the (row, choice) pairs in order of expert, within an expert in order of row, take slots 0, 1, ..;
+ *   offsets [n_experts + 1]: first slot of every expert, slot_of [n_rows, top_k] (-1: none), row_of [n_rows * top_k] (-1 behind the last).
+ * bwd: dlogits from the gradients of the weights and of the loss (either NULL: zero); ids, weights, counts as fwd gave them.
+ * n_experts <= 1024, top_k <= 32, n_rows * top_k < 2^31.  A NaN logit ranks above all numbers and makes its row's weights and the loss NaN. */
+typedef struct mb_route {
+  int64_t n_rows;
+  int32_t n_experts, top_k, dtype, renorm;                /* dtype of logits and dlogits */
+  const void* logits; int64_t ld_logits;
+  const uint8_t* valid;                                   /* [n_rows] or NULL */
+  int32_t* ids; float* weights;                           /* [n_rows, top_k] */
+  int32_t* counts; float* loss;
+  int32_t *offsets, *row_of, *slot_of;
+  const float *dweights, *dloss;
+  void* dlogits; int64_t ld_dlogits;
+  void* scratch;                                          /* fwd: mb_route_scratch() bytes */
+} mb_route;
+size_t mb_route_scratch(int64_t n_rows, int32_t n_experts);
+int mb_route_fwd(const mb_route* d, void* stream);
+int mb_route_bwd(const mb_route* d, void* stream);
+
+/* The experts' dense layers on grouped rows: slot s of expert e (offsets[e] <= s < offsets[e+1])
+ *   y[s] = act(f(x[idx[s]]) W_e^T + bias_e) [* SiLU'(gate[s])]       W [n_experts, n_out, n_in], bias [n_experts, n_out]
+ * idx NULL: row s itself; in_act: f = SiLU.  Widths are multiples of 128, at most 1024; rows 16-byte aligned.
+ * Slots behind offsets[n_experts] are left as they are, or set to zero with zero_rest.  Offsets and idx are cut to their ranges.
+ * The data gradient is the same call on the transposed weights.
+ * grad_w: dw_e = sum_s dy[s]^T f(x[idx[s]]), dbias_e = sum_s dy[s] (dbias NULL: not wanted), summed in a fixed order. */
+typedef struct mb_experts {
+  int64_t n_slots, n_rows;                                /* n_rows: rows of x */
+  int32_t n_experts, n_in, n_out, in_act, out_act, zero_rest;
+  const int32_t *offsets, *idx;
+  const float* x; int64_t ld_x;
+  const float* w;
+  const float* w_lo;                                      /* w less its 11 leading bits (mb_experts_split) */
+  const float* bias;
+  const float* gate; int64_t ld_gate;
+  float* y; int64_t ld_y;
+  const float* dy; int64_t ld_dy;
+  float* dw; float* dbias;
+  void* scratch;                                          /* grad_w: mb_experts_grad_scratch() bytes */
+} mb_experts;
+int mb_experts_linear(const mb_experts* d, void* stream);
+size_t mb_experts_grad_scratch(int64_t n_slots, int32_t n_experts, int32_t n_in, int32_t n_out);
+int mb_experts_grad_w(const mb_experts* d, void* stream);
+
+/* out[t] = sum_j weights[t,j] y[slot_of[t,j]] over the choices j with a slot (weights NULL: 1); width a multiple of 4.
+ * bwd: dy[slot_of[t,j]] = weights[t,j] dout[t], dweights[t,j] = dout[t] . y[slot_of[t,j]] (0 without a slot; NULL: not wanted); dy rows
+ * from offsets[n_experts] on are set to zero where offsets is given. */
+typedef struct mb_combine {
+  int64_t n_rows, n_slots;
+  int32_t top_k, width, n_experts, pad0;
+  const int32_t *slot_of, *offsets;
+  const float* weights;
+  const float* y; int64_t ld_y;
+  float* out; int64_t ld_out;
+  const float* dout; int64_t ld_dout;
+  float* dy; int64_t ld_dy;
+  float* dweights;
+} mb_combine;
+int mb_experts_combine_fwd(const mb_combine* d, void* stream);
+int mb_experts_combine_bwd(const mb_combine* d, void* stream);
+
 /* embedding lookup: y[r] = table[idx[r] + offset] (nn.Embedding, matris/model/feature_embed.py:37) */
 int mb_embedding(int64_t n_rows, const int32_t* idx, int32_t offset, const float* table, float* y, void* stream);
 

@@ -152,6 +152,40 @@ class MbOpRecord(C.Structure):
                 ("rows", _i64), ("k", _i32), ("n", _i32)]
 
 
+class MbGroupNorm(C.Structure):
+    _fields_ = [
+        ("n_rows", _i64), ("n_seg", _i32), ("channels", _i32), ("groups", _i32), ("dtype", _i32), ("act", _i32), ("zero_rest", _i32),
+        ("eps", _f32), ("pad0", _i32), ("seg_ptr", _vp), ("x", _vp), ("ld_x", _i64), ("weight", _vp), ("bias", _vp),
+        ("y", _vp), ("ld_y", _i64), ("stats", _vp), ("dy", _vp), ("ld_dy", _i64), ("dx", _vp), ("ld_dx", _i64),
+        ("dweight", _vp), ("dbias", _vp), ("scratch", _vp),
+    ]
+
+
+class MbRoute(C.Structure):
+    _fields_ = [
+        ("n_rows", _i64), ("n_experts", _i32), ("top_k", _i32), ("dtype", _i32), ("renorm", _i32), ("logits", _vp), ("ld_logits", _i64),
+        ("valid", _vp), ("ids", _vp), ("weights", _vp), ("counts", _vp), ("loss", _vp), ("offsets", _vp), ("row_of", _vp),
+        ("slot_of", _vp), ("dweights", _vp), ("dloss", _vp), ("dlogits", _vp), ("ld_dlogits", _i64), ("scratch", _vp),
+    ]
+
+
+class MbExperts(C.Structure):
+    _fields_ = [
+        ("n_slots", _i64), ("n_rows", _i64), ("n_experts", _i32), ("n_in", _i32), ("n_out", _i32), ("in_act", _i32), ("out_act", _i32),
+        ("zero_rest", _i32), ("offsets", _vp), ("idx", _vp), ("x", _vp), ("ld_x", _i64), ("w", _vp), ("w_lo", _vp), ("bias", _vp),
+        ("gate", _vp), ("ld_gate", _i64), ("y", _vp), ("ld_y", _i64), ("dy", _vp), ("ld_dy", _i64), ("dw", _vp), ("dbias", _vp),
+        ("scratch", _vp),
+    ]
+
+
+class MbCombine(C.Structure):
+    _fields_ = [
+        ("n_rows", _i64), ("n_slots", _i64), ("top_k", _i32), ("width", _i32), ("n_experts", _i32), ("pad0", _i32), ("slot_of", _vp),
+        ("offsets", _vp), ("weights", _vp), ("y", _vp), ("ld_y", _i64), ("out", _vp), ("ld_out", _i64), ("dout", _vp), ("ld_dout", _i64),
+        ("dy", _vp), ("ld_dy", _i64), ("dweights", _vp),
+    ]
+
+
 # name -> argtypes (every function returns int status unless listed in _OTHER)
 _SIGNATURES = {
     "mb_cell_grid": [_i64, _vp, _vp, C.c_double, _vp, _vp, C.POINTER(_i64)],
@@ -188,6 +222,14 @@ _SIGNATURES = {
     "mb_layernorm_bwd": [_i64, _vp, _vp, _vp, _vp, _vp],
     "mb_rmsnorm_fwd": [_i64, _vp, _vp, _vp, _vp],
     "mb_rmsnorm_bwd": [_i64, _vp, _vp, _vp, _vp, _vp],
+    "mb_group_norm_fwd": [C.POINTER(MbGroupNorm), _vp],
+    "mb_group_norm_bwd": [C.POINTER(MbGroupNorm), _vp],
+    "mb_route_fwd": [C.POINTER(MbRoute), _vp],
+    "mb_route_bwd": [C.POINTER(MbRoute), _vp],
+    "mb_experts_linear": [C.POINTER(MbExperts), _vp],
+    "mb_experts_grad_w": [C.POINTER(MbExperts), _vp],
+    "mb_experts_combine_fwd": [C.POINTER(MbCombine), _vp],
+    "mb_experts_combine_bwd": [C.POINTER(MbCombine), _vp],
     "mb_embedding": [_i64, _vp, _i32, _vp, _vp, _vp],
     "mb_head_dot_fwd": [_i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp],
     "mb_head_dot_bwd": [_i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp],
@@ -216,6 +258,9 @@ _OTHER = {
     "mb_status_string": (C.c_char_p, [C.c_int]),
     "mb_last_cuda_error": (C.c_char_p, []),
     "mb_graph_scan_tmp_len": (C.c_size_t, [_i64]),
+    "mb_group_norm_scratch": (C.c_size_t, [_i64, _i32, _i32]),
+    "mb_route_scratch": (C.c_size_t, [_i64, _i32]),
+    "mb_experts_grad_scratch": (C.c_size_t, [_i64, _i32, _i32, _i32]),
 }
 
 _lib = None

@@ -6,7 +6,9 @@ wrapper launches on torch's current stream.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import struct
+from typing import NamedTuple
 
 import torch
 
@@ -444,6 +446,351 @@ def segment_sum_scalar(n_seg, seg_ptr, x):
     out = torch.empty(n_seg, dtype=torch.float32, device=x.device)
     call("mb_segment_sum_scalar", n_seg, ptr(seg_ptr), ptr(x), ptr(out), _stream())
     return out
+
+
+# ------------------------------------------------------------------ group norm and mixture of experts
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _take(t, name, dtype, shape=None, dense=True):
+    """Check one argument: element type, shape (None: any size), layout.  The device is checked last (``_here``)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a tensor is wanted, got {type(t).__name__}")
+    if t.dtype not in (dtype if isinstance(dtype, (tuple, dict)) else (dtype,)):
+        raise TypeError(f"{name}: element type {t.dtype}")
+    if shape is not None and (t.dim() != len(shape) or any(w is not None and w != h for w, h in zip(shape, t.shape))):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, {tuple('any' if w is None else w for w in shape)} is wanted")
+    if dense and not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous tensor is wanted, got strides {t.stride()}")
+    return t
+
+
+def _row_stride(t, name):
+    """Row stride of a [rows, width] tensor whose rows are contiguous and do not overlap."""
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the values of a row have to be neighbours, got strides {t.stride()}")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name}: rows overlap, got strides {t.stride()}")
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _aligned_rows(t, name):
+    """``_row_stride`` of rows that are read in 16-byte pieces."""
+    ld = _row_stride(t, name)
+    if t.data_ptr() % 16 or (t.shape[0] > 1 and ld * t.element_size() % 16):
+        raise ValueError(f"{name}: rows have to start on 16-byte boundaries")
+    return ld
+
+
+def _here(**tensors):
+    """The launches go to the current device: every tensor has to be there."""
+    for name, t in tensors.items():
+        if t is not None and (t.device.type != "cuda" or t.device.index != torch.cuda.current_device()):
+            raise ValueError(f"{name} is on {t.device}: it has to be on the current CUDA device")
+
+
+def _norm_rows(x, weight, bias, seg_ptr, n_groups, act, eps):
+    """[rows, channels] view, row stride and number of segments of a group norm's input."""
+    _take(x, "x", _DTYPES, dense=False)
+    if seg_ptr is None:
+        if x.dim() < 2:
+            raise ValueError("x: [batch, .., channels] is wanted without seg_ptr")
+        if not x.is_contiguous():
+            raise ValueError(f"x: a contiguous tensor is wanted without seg_ptr, got strides {x.stride()}")
+        n_seg, x = x.shape[0], x.view(math.prod(x.shape[:-1]), x.shape[-1])
+    else:
+        _take(x, "x", _DTYPES, (None, None), dense=False)
+        n_seg = _take(seg_ptr, "seg_ptr", torch.int32, (None,)).shape[0] - 1
+        if n_seg < 0:
+            raise ValueError("seg_ptr: [segments + 1] offsets are wanted, got none")
+    channels = x.shape[1]
+    if not 1 <= channels <= 1024:
+        raise NotImplementedError(f"group norm takes 1 to 1024 channels, got {channels}")
+    if n_groups < 1 or channels % n_groups:
+        raise ValueError(f"{channels} channels do not divide into {n_groups} groups")
+    if act not in (0, 1):
+        raise ValueError(f"act={act!r}: 0 (none) or 1 (SiLU)")
+    if not eps > 0:
+        raise ValueError(f"eps={eps!r} has to be positive")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _take(t, name, torch.float32, (channels,))
+    _row_stride(x, "x")
+    if x.shape[0] >= 1 << 31:
+        raise NotImplementedError("group norm takes fewer than 2**31 rows")
+    return x, n_seg
+
+
+def _norm_desc(x, weight, bias, n_groups, n_seg, seg_ptr, eps, act, stats):
+    d = _lib.MbGroupNorm()
+    d.n_rows, d.n_seg, d.channels, d.groups = x.shape[0], n_seg, x.shape[1], n_groups
+    d.dtype, d.act, d.eps = _DTYPES[x.dtype], act, eps
+    d.weight, d.bias, d.seg_ptr, d.x, d.ld_x, d.stats = ptr(weight), ptr(bias), ptr(seg_ptr), ptr(x), _row_stride(x, "x"), ptr(stats)
+    return d
+
+
+def _norm_out(x, x_given, out, name):
+    """The output rows (same shape and type as the input) and whether rows of no segment are to be cleared."""
+    if out is None:
+        return torch.empty(x_given.shape, dtype=x.dtype, device=x.device), True
+    _take(out, name, x.dtype, tuple(x_given.shape), dense=x_given.dim() != 2)
+    return out, False
+
+
+def group_norm_fwd(x, weight, bias, n_groups, seg_ptr=None, eps=1e-5, act=0, out=None):
+    """Group norm with an optional SiLU (``act=1``), features last: every segment of rows and group of neighbouring channels
+    has its own mean and variance (float32 arithmetic; x float32, bfloat16 or float16; weight and bias float32 [channels] or None).
+
+    ``x`` [rows, channels] with ``seg_ptr`` (int32 [segments + 1] row offsets on the device, as a batch's ``atom_ptr``), or
+    [batch, .., channels] without.  Returns (y, stats): stats [segments, groups, 2] (mean, 1 / deviation) is what
+    ``group_norm_bwd`` reads.  Rows of no segment are zero in a returned tensor and left alone in a given ``out``, which may be x."""
+    rows, n_seg = _norm_rows(x, weight, bias, seg_ptr, n_groups, act, eps)
+    y, zero = _norm_out(rows, x, out, "out")
+    _here(x=x, weight=weight, bias=bias, seg_ptr=seg_ptr, out=out)
+    if zero and n_seg == 0:
+        y.zero_()
+    stats = new(n_seg * n_groups, 2, x, zero=not rows.shape[0]).view(n_seg, n_groups, 2)
+    d = _norm_desc(rows, weight, bias, n_groups, n_seg, seg_ptr, eps, act, stats)
+    yr = y if seg_ptr is not None else y.view(rows.shape)
+    d.y, d.ld_y, d.zero_rest = ptr(yr), _row_stride(yr, "out"), int(zero)
+    scratch = torch.empty(_lib.load().mb_group_norm_scratch(d.n_rows, n_seg, d.channels), dtype=torch.uint8, device=x.device)
+    d.scratch = ptr(scratch)
+    call("mb_group_norm_fwd", C.byref(d), _stream())
+    return y, stats
+
+
+def group_norm_bwd(dy, x, weight, bias, stats, n_groups, seg_ptr=None, act=0, out=None, want_affine=True):
+    """Gradients (dx, dweight, dbias) of ``group_norm_fwd`` from its inputs and ``stats``; dweight and dbias are None unless
+    ``want_affine``.  dx is written to ``out`` where given (it may be dy or x)."""
+    rows, n_seg = _norm_rows(x, weight, bias, seg_ptr, n_groups, act, 1.0)
+    _take(dy, "dy", x.dtype, tuple(x.shape), dense=seg_ptr is None)
+    _take(stats, "stats", torch.float32, (n_seg, n_groups, 2))
+    dx, zero = _norm_out(rows, x, out, "out")
+    _here(x=x, dy=dy, weight=weight, bias=bias, stats=stats, seg_ptr=seg_ptr, out=out)
+    if zero and n_seg == 0:
+        dx.zero_()
+    d = _norm_desc(rows, weight, bias, n_groups, n_seg, seg_ptr, 1.0, act, stats)
+    dyr, dxr = (dy, dx) if seg_ptr is not None else (dy.view(rows.shape), dx.view(rows.shape))
+    d.dy, d.ld_dy, d.dx, d.ld_dx, d.zero_rest = ptr(dyr), _row_stride(dyr, "dy"), ptr(dxr), _row_stride(dxr, "out"), int(zero)
+    dweight = dbias = None
+    if want_affine:
+        dweight, dbias = torch.empty(2, d.channels, dtype=torch.float32, device=x.device).unbind(0)
+        d.dweight, d.dbias = ptr(dweight), ptr(dbias)
+    scratch = torch.empty(_lib.load().mb_group_norm_scratch(d.n_rows, n_seg, d.channels), dtype=torch.uint8, device=x.device)
+    d.scratch = ptr(scratch)
+    call("mb_group_norm_bwd", C.byref(d), _stream())
+    return dx, dweight, dbias
+
+
+class Route(NamedTuple):
+    """What ``route_fwd`` returns: choices and weights of every row [rows, top_k], the balance loss (scalar), the rows that took
+    every expert, and the grouping of the (row, choice) pairs by expert (``offsets``, ``row_of``, ``slot_of``)."""
+
+    ids: torch.Tensor
+    weights: torch.Tensor
+    loss: torch.Tensor
+    totals: torch.Tensor  # [experts + 1]: rows of every expert, rows routed
+    offsets: torch.Tensor
+    row_of: torch.Tensor
+    slot_of: torch.Tensor
+    renorm: bool
+
+    @property
+    def counts(self):
+        return self.totals[:-1]
+
+
+def _route_desc(logits, top_k, renorm):
+    _take(logits, "logits", _DTYPES, (None, None), dense=False)
+    n, n_experts = logits.shape
+    if not 1 <= n_experts <= 1024:
+        raise NotImplementedError(f"the router takes 1 to 1024 experts, got {n_experts}")
+    if not 1 <= top_k <= min(32, n_experts):
+        raise ValueError(f"top_k={top_k}: 1 to {min(32, n_experts)} of {n_experts} experts")
+    if n * top_k >= 1 << 31:
+        raise NotImplementedError("the router takes fewer than 2**31 choices")
+    d = _lib.MbRoute()
+    d.n_rows, d.n_experts, d.top_k, d.dtype, d.renorm = n, n_experts, top_k, _DTYPES[logits.dtype], int(renorm)
+    d.logits, d.ld_logits = ptr(logits), _row_stride(logits, "logits")
+    return d
+
+
+def route_fwd(logits, top_k, valid=None, renorm=True) -> Route:
+    """Router of a mixture of experts.  p = softmax over a row's available experts (logit > -inf); the ``top_k`` largest are
+    taken, equal ones by the lowest index; weights p, or p over their sum with ``renorm``.  ``valid`` [rows] bool: False rows are
+    padding.  Padding and rows without an available expert have ids -1, weights 0 and no slot, and count nowhere.
+
+    loss = experts / (top_k T^2) sum_e counts_e sum_rows p_e with T the rows routed: 1 where both are even.  Slots 0, 1, ..
+    hold the pairs in order of expert, then of row: expert e has slots offsets[e] .. offsets[e+1] - 1, slot s is of row row_of[s]
+    (-1 behind the last), choice j of row t has slot slot_of[t, j]."""
+    d = _route_desc(logits, top_k, renorm)
+    n, n_experts = logits.shape
+    if valid is not None:
+        _take(valid, "valid", torch.bool, (n,))
+    _here(logits=logits, valid=valid)
+    dev = logits.device
+    ints = torch.empty(2 * n_experts + 2, dtype=torch.int32, device=dev)
+    ids, slot_of, row_of = torch.empty(3, n * top_k, dtype=torch.int32, device=dev).unbind(0)
+    weights, loss = torch.empty(n, top_k, dtype=torch.float32, device=dev), torch.empty((), dtype=torch.float32, device=dev)
+    totals, offsets = ints[:n_experts + 1], ints[n_experts + 1:]
+    scratch = torch.empty(_lib.load().mb_route_scratch(n, n_experts), dtype=torch.uint8, device=dev)
+    d.valid, d.ids, d.weights, d.counts, d.loss = ptr(valid), ptr(ids), ptr(weights), ptr(totals), ptr(loss)
+    d.offsets, d.row_of, d.slot_of, d.scratch = ptr(offsets), ptr(row_of), ptr(slot_of), ptr(scratch)
+    call("mb_route_fwd", C.byref(d), _stream())
+    return Route(ids.view(n, top_k), weights, loss, totals, offsets, row_of, slot_of.view(n, top_k), bool(renorm))
+
+
+def route_bwd(logits, route: Route, dweights=None, dloss=None):
+    """Gradient of the logits from those of the weights [rows, top_k] and of the balance loss (a scalar tensor); None: zero."""
+    n, top_k = route.ids.shape
+    d = _route_desc(logits, top_k, route.renorm)
+    _take(route.ids, "route.ids", torch.int32, (logits.shape[0], top_k))
+    _take(route.weights, "route.weights", torch.float32, (n, top_k))
+    _take(route.totals, "route.totals", torch.int32, (logits.shape[1] + 1,))
+    if dweights is not None:
+        _take(dweights, "dweights", torch.float32, (n, top_k))
+    if dloss is not None and _take(dloss, "dloss", torch.float32).numel() != 1:
+        raise ValueError(f"dloss: a scalar is wanted, got shape {tuple(dloss.shape)}")
+    _here(logits=logits, ids=route.ids, weights=route.weights, totals=route.totals, dweights=dweights, dloss=dloss)
+    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    d.ids, d.weights, d.counts, d.dweights, d.dloss = ptr(route.ids), ptr(route.weights), ptr(route.totals), ptr(dweights), ptr(dloss)
+    d.dlogits, d.ld_dlogits = ptr(dlogits), logits.shape[1]
+    call("mb_route_bwd", C.byref(d), _stream())
+    return dlogits
+
+
+class ExpertWeights:
+    """Weights [experts, n_out, n_in] of the experts' dense layers, laid out once for ``experts_linear`` in both directions."""
+
+    __slots__ = ("w", "wt")
+
+    def __init__(self, w: torch.Tensor):
+        w = _take(w.detach(), "weights", torch.float32, (None, None, None), dense=False).contiguous()
+        if not 1 <= w.shape[0] <= 1024:
+            raise NotImplementedError(f"1 to 1024 experts, got {w.shape[0]}")
+        _expert_widths(w.shape[2], w.shape[1])
+        _here(weights=w)
+        self.w, self.wt = w, w.transpose(1, 2).contiguous()
+
+
+def _expert_widths(n_in, n_out):
+    for n in (n_in, n_out):
+        if n % D or not D <= n <= 1024:
+            raise NotImplementedError(f"the experts' kernels take widths 128, 256 .. 1024, got {n_in} -> {n_out}")
+
+
+def _experts_desc(x, offsets, idx, n_in, n_out, in_act):
+    _take(x, "x", torch.float32, (None, n_in), dense=False)
+    _take(offsets, "offsets", torch.int32, (None,))
+    d = _lib.MbExperts()
+    d.n_rows = d.n_slots = x.shape[0]
+    if idx is not None:
+        d.n_slots = _take(idx, "idx", torch.int32, (None,)).shape[0]
+        if d.n_slots and not d.n_rows:
+            raise ValueError("idx: there are no rows to take")
+    if d.n_slots >= 1 << 31:
+        raise NotImplementedError("fewer than 2**31 slots")
+    if in_act not in (0, 1):
+        raise ValueError(f"in_act={in_act!r}: 0 (none) or 1 (SiLU)")
+    d.n_experts, d.n_in, d.n_out, d.in_act = offsets.shape[0] - 1, n_in, n_out, in_act
+    d.offsets, d.idx, d.x, d.ld_x = ptr(offsets), ptr(idx), ptr(x), _aligned_rows(x, "x")
+    return d
+
+
+def experts_linear(x, weights, offsets, bias=None, idx=None, in_act=0, out_act=0, gate=None, transposed=False, out=None):
+    """Dense layers of a mixture of experts on rows grouped by expert: for the slots s of expert e
+    y[s] = act(f(x[idx[s]]) W_e^T + bias_e), times SiLU'(gate[s]) where ``gate`` [slots, n_out] is given (idx None: row s itself).
+
+    ``weights``: ExpertWeights, or a [experts, n_out, n_in] tensor that is laid out in the call; ``transposed``: W_e in the place
+    of its transpose, the data gradient.  ``in_act`` / ``out_act`` 1: SiLU.  ``offsets``, ``idx``: ``Route.offsets``, ``Route.row_of``.
+    Slots behind the last are zero in a returned tensor and left alone in a given ``out``."""
+    if not isinstance(weights, ExpertWeights):
+        weights = ExpertWeights(weights)
+    w = weights.wt if transposed else weights.w
+    n_experts, n_out, n_in = w.shape
+    d = _experts_desc(x, offsets, idx, n_in, n_out, in_act)
+    if d.n_experts != n_experts:
+        raise ValueError(f"offsets: [{n_experts + 1}] is wanted, got {tuple(offsets.shape)}")
+    if out_act not in (0, 1):
+        raise ValueError(f"out_act={out_act!r}: 0 (none) or 1 (SiLU)")
+    if bias is not None:
+        _take(bias, "bias", torch.float32, (n_experts, n_out))
+    if gate is not None:
+        _take(gate, "gate", torch.float32, (d.n_slots, n_out), dense=False)
+        d.gate, d.ld_gate = ptr(gate), _aligned_rows(gate, "gate")
+    if out is not None:
+        _take(out, "out", torch.float32, (d.n_slots, n_out), dense=False)
+    _here(x=x, weights=w, offsets=offsets, bias=bias, idx=idx, gate=gate, out=out)
+    y = new(d.n_slots, n_out, x) if out is None else out
+    d.w, d.bias, d.out_act, d.zero_rest = ptr(w), ptr(bias), out_act, int(out is None)
+    d.y, d.ld_y = ptr(y), _aligned_rows(y, "out")
+    call("mb_experts_linear", C.byref(d), _stream())
+    return y
+
+
+def experts_grad_w(dy, x, offsets, idx=None, in_act=0, want_bias=True):
+    """Weight gradients of ``experts_linear``: (dW [experts, n_out, n_in], dbias [experts, n_out] or None) with
+    dW_e = sum over the slots of e of dy[s]^T f(x[idx[s]]), summed in a fixed order.  An expert without slots has zeros."""
+    _take(dy, "dy", torch.float32, (None, None), dense=False)
+    if x.dim() != 2:
+        raise ValueError(f"x: [rows, n_in] is wanted, got shape {tuple(x.shape)}")
+    _expert_widths(x.shape[1], dy.shape[1])
+    d = _experts_desc(x, offsets, idx, x.shape[1], dy.shape[1], in_act)
+    if dy.shape[0] != d.n_slots:
+        raise ValueError(f"dy: {d.n_slots} slots are wanted, got {dy.shape[0]}")
+    if not 1 <= d.n_experts <= 1024:
+        raise NotImplementedError(f"1 to 1024 experts, got {d.n_experts}")
+    d.dy, d.ld_dy = ptr(dy), _aligned_rows(dy, "dy")
+    _here(dy=dy, x=x, offsets=offsets, idx=idx)
+    dw = torch.empty(d.n_experts, d.n_out, d.n_in, dtype=torch.float32, device=x.device)
+    dbias = torch.empty(d.n_experts, d.n_out, dtype=torch.float32, device=x.device) if want_bias else None
+    scratch = torch.empty(_lib.load().mb_experts_grad_scratch(d.n_slots, d.n_experts, d.n_in, d.n_out), dtype=torch.uint8, device=x.device)
+    d.dw, d.dbias, d.scratch = ptr(dw), ptr(dbias), ptr(scratch)
+    call("mb_experts_grad_w", C.byref(d), _stream())
+    return dw, dbias
+
+
+def _combine_desc(y, slot_of, weights):
+    _take(y, "y", torch.float32, (None, None), dense=False)
+    n, k = _take(slot_of, "slot_of", torch.int32, (None, None)).shape
+    if y.shape[1] % 4 or not y.shape[1]:
+        raise NotImplementedError(f"widths that are multiples of 4, got {y.shape[1]}")
+    if k < 1 or n * k >= 1 << 31 or y.shape[0] >= 1 << 31:
+        raise NotImplementedError(f"1 choice a row or more, fewer than 2**31 in all, got {n} x {k}")
+    if weights is not None:
+        _take(weights, "weights", torch.float32, (n, k))
+    d = _lib.MbCombine()
+    d.n_rows, d.n_slots, d.top_k, d.width = n, y.shape[0], k, y.shape[1]
+    d.slot_of, d.weights, d.y, d.ld_y = ptr(slot_of), ptr(weights), ptr(y), _aligned_rows(y, "y")
+    return d
+
+
+def experts_combine_fwd(y, slot_of, weights=None):
+    """The experts' outputs back to their rows: out[t] = sum_j weights[t, j] y[slot_of[t, j]] over the choices with a slot
+    (weights None: 1, the sum that the gradient of the gathered rows takes)."""
+    d = _combine_desc(y, slot_of, weights)
+    _here(y=y, slot_of=slot_of, weights=weights)
+    out = new(d.n_rows, d.width, y)
+    d.out, d.ld_out = ptr(out), d.width
+    call("mb_experts_combine_fwd", C.byref(d), _stream())
+    return out
+
+
+def experts_combine_bwd(dout, y, slot_of, weights=None, offsets=None):
+    """Gradients (dy, dweights) of ``experts_combine_fwd``: dy [slots, width], dweights [rows, top_k] (0 for a choice without a
+    slot).  Slots that no choice has are zero from ``offsets[-1]`` on; without ``offsets`` every slot has to have its choice."""
+    d = _combine_desc(y, slot_of, weights)
+    _take(dout, "dout", torch.float32, (d.n_rows, d.width), dense=False)
+    if offsets is not None:
+        d.n_experts, d.offsets = _take(offsets, "offsets", torch.int32, (None,)).shape[0] - 1, ptr(offsets)
+        if d.n_experts < 0:
+            raise ValueError("offsets: [experts + 1] is wanted, got none")
+    d.dout, d.ld_dout = ptr(dout), _aligned_rows(dout, "dout")
+    _here(dout=dout, y=y, slot_of=slot_of, weights=weights, offsets=offsets)
+    dy, dweights = new(d.n_slots, d.width, y), new(d.n_rows, d.top_k, y)
+    d.dy, d.ld_dy, d.dweights = ptr(dy), d.width, ptr(dweights)
+    call("mb_experts_combine_bwd", C.byref(d), _stream())
+    return dy, dweights
 
 
 # ------------------------------------------------------------------ geometry and bases
