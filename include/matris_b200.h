@@ -466,15 +466,16 @@ int mb_route_bwd(const mb_route* d, void* stream);
  *   y[s] = act(f(x[idx[s]]) W_e^T + bias_e) [* SiLU'(gate[s])]       W [n_experts, n_out, n_in], bias [n_experts, n_out]
  * idx NULL: row s itself; in_act: f = SiLU.  Widths are multiples of 128, at most 1024; rows 16-byte aligned.
  * Slots behind offsets[n_experts] are left as they are, or set to zero with zero_rest.  Offsets and idx are cut to their ranges.
- * The data gradient is the same call on the transposed weights.
+ * The data gradient is the same call on the transposed parts, n_in and n_out exchanged.
+ * split: parts [4, n_experts * n_out * n_in] = hi and lo of w (w = hi + lo, hi of 11 significant bits), hi and lo of every expert's
+ * transpose [n_in, n_out]; 16-byte aligned.
  * grad_w: dw_e = sum_s dy[s]^T f(x[idx[s]]), dbias_e = sum_s dy[s] (dbias NULL: not wanted), summed in a fixed order. */
 typedef struct mb_experts {
   int64_t n_slots, n_rows;                                /* n_rows: rows of x */
   int32_t n_experts, n_in, n_out, in_act, out_act, zero_rest;
   const int32_t *offsets, *idx;
   const float* x; int64_t ld_x;
-  const float* w;
-  const float* w_lo;                                      /* w less its 11 leading bits (mb_experts_split) */
+  const float *w_hi, *w_lo;                               /* linear: two of the parts that mb_experts_split wrote */
   const float* bias;
   const float* gate; int64_t ld_gate;
   float* y; int64_t ld_y;
@@ -482,6 +483,7 @@ typedef struct mb_experts {
   float* dw; float* dbias;
   void* scratch;                                          /* grad_w: mb_experts_grad_scratch() bytes */
 } mb_experts;
+int mb_experts_split(int32_t n_experts, int32_t n_out, int32_t n_in, const float* w, float* parts, void* stream);
 int mb_experts_linear(const mb_experts* d, void* stream);
 size_t mb_experts_grad_scratch(int64_t n_slots, int32_t n_experts, int32_t n_in, int32_t n_out);
 int mb_experts_grad_w(const mb_experts* d, void* stream);

@@ -172,7 +172,7 @@ class MbRoute(C.Structure):
 class MbExperts(C.Structure):
     _fields_ = [
         ("n_slots", _i64), ("n_rows", _i64), ("n_experts", _i32), ("n_in", _i32), ("n_out", _i32), ("in_act", _i32), ("out_act", _i32),
-        ("zero_rest", _i32), ("offsets", _vp), ("idx", _vp), ("x", _vp), ("ld_x", _i64), ("w", _vp), ("w_lo", _vp), ("bias", _vp),
+        ("zero_rest", _i32), ("offsets", _vp), ("idx", _vp), ("x", _vp), ("ld_x", _i64), ("w_hi", _vp), ("w_lo", _vp), ("bias", _vp),
         ("gate", _vp), ("ld_gate", _i64), ("y", _vp), ("ld_y", _i64), ("dy", _vp), ("ld_dy", _i64), ("dw", _vp), ("dbias", _vp),
         ("scratch", _vp),
     ]
@@ -226,6 +226,7 @@ _SIGNATURES = {
     "mb_group_norm_bwd": [C.POINTER(MbGroupNorm), _vp],
     "mb_route_fwd": [C.POINTER(MbRoute), _vp],
     "mb_route_bwd": [C.POINTER(MbRoute), _vp],
+    "mb_experts_split": [_i32, _i32, _i32, _vp, _vp, _vp],
     "mb_experts_linear": [C.POINTER(MbExperts), _vp],
     "mb_experts_grad_w": [C.POINTER(MbExperts), _vp],
     "mb_experts_combine_fwd": [C.POINTER(MbCombine), _vp],

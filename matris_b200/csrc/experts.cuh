@@ -1,0 +1,392 @@
+// Dense layers of a mixture of experts on rows grouped by expert: forward and data gradient (one product), weight gradient.
+// (Included by gemm.cu inside namespace mb, after its tensor-core helpers and k_gemm_ps.)
+
+constexpr int EX_MAX_EXPERTS = 1024, EX_MAX_WIDTH = 1024;
+
+// Slots of an expert, whatever the offsets hold
+__device__ __forceinline__ void expert_slots(const mb_experts& d, int e, int64_t& from, int64_t& to) {
+  from = min(max((int64_t)d.offsets[e], (int64_t)0), d.n_slots);
+  to = min(max((int64_t)d.offsets[e + 1], from), d.n_slots);
+}
+__device__ __forceinline__ const float* source_row(const mb_experts& d, int64_t s) {
+  const int64_t r = d.idx ? min(max((int64_t)d.idx[s], (int64_t)0), d.n_rows - 1) : s;
+  return d.x + r * d.ld_x;
+}
+
+// ------------------------------------------------------------------ forward and data gradient
+// y[s] = act(f(x[idx[s]]) W_e^T + b_e) on the tensor cores: the roles of k_gemm_ps (which see) on row tiles that belong to one expert each.
+//
+// Row tiles are numbered through the experts, ceil(slots / 128) of them each; a warp finds a tile's expert with one scan over 32
+// experts' counts at a time (Walk), from the offsets on the device, so that the host never reads them.  A tile's rows are gathered
+// through idx, its weights are rows e n_out + 128 j .. of one tensor map over all experts' weights.  Rows behind the expert's last slot
+// repeat it and are not stored: the next expert's rows belong to another tile.
+//
+// Operands are split into two tf32 parts, both rounded to nearest: x = hi + lo to 2^-23, and the three products kept drop lo lo,
+// at most 2^-22 of |x w| and of either sign: the float32 rounding of the sums is as large.  (Two bf16 parts, as the other dense
+// layers have, are twice as fast and good to 2^-17: of no use here, where memory bounds the call either way.)
+//
+// shared (K = 128): the four A buffers hold the whole row tile, converted once for all its column blocks.  Otherwise a column block is a
+// tile of its own and its rows are gathered again, from L2.
+struct alignas(64) ExMaps { CUtensorMap hi, lo; };
+
+// Tiles of 128 slots in order of expert; all lanes of a warp call it together
+struct Walk {
+  const mb_experts* d;
+  int base, before, total;   // first expert held (lane l: base + l), tiles ahead of it, tiles of the 32
+  int64_t from, to;
+  int upto;                  // tiles of this and the lower lanes' experts
+  __device__ __forceinline__ void load() {
+    const int lane = threadIdx.x & 31, e = base + lane;
+    from = to = 0;
+    if (e < d->n_experts) expert_slots(*d, e, from, to);
+    upto = (int)((to - from + 127) >> 7);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    total = __shfl_sync(0xffffffffu, upto, 31);
+  }
+  __device__ __forceinline__ void start(const mb_experts& args) { d = &args; base = before = 0; load(); }
+  // tile t (never less than the last one asked for): its expert, first slot and number of slots; false: there are no more
+  __device__ __forceinline__ bool seek(int t, int& e, int64_t& s0, int& rows) {
+    while (t - before >= total) {
+      before += total;
+      base += 32;
+      if (base >= d->n_experts) { total = before = 0; return false; }
+      load();
+    }
+    const int at = __popc(__ballot_sync(0xffffffffu, t - before >= upto));
+    const int ahead = __shfl_sync(0xffffffffu, upto, at > 0 ? at - 1 : 0), first = at > 0 ? ahead : 0;
+    e = base + at;
+    s0 = __shfl_sync(0xffffffffu, from, at) + (int64_t)(t - before - first) * 128;
+    const int64_t left = __shfl_sync(0xffffffffu, to, at) - s0;
+    rows = left < 128 ? (int)left : 128;
+    return true;
+  }
+};
+
+constexpr int EX_STAGES = 3;                                     // patches of a producer warp
+constexpr int EX_PATCH_BYTES = 8 * EX_STAGES * 32 * 128;
+constexpr int EX_BAR_OFF = PS_RING_BYTES + EX_PATCH_BYTES;
+constexpr int EX_SMEM_BYTES = EX_BAR_OFF + 256;
+static_assert(EX_SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
+
+__device__ __forceinline__ float rest_tf32(float x, float hi) { return to_tf32(x - hi); }
+
+__global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant__ mb_experts d, const __grid_constant__ ExMaps maps, const int shared) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + EX_BAR_OFF);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + EX_BAR_OFF + 240);
+  if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need a 1024-byte aligned base
+    if (threadIdx.x == 0) atomicOr(&g_gemm_status, 2);
+    return;
+  }
+  // a_ready[4] (4 producer warps) a_done[4] | w_ready[4] w_done[4] | d_full[2] d_free[2] (8 epilogue warps) | retired
+  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t a_ready = bar0, a_done = bar0 + 32, w_ready = bar0 + 64, w_done = bar0 + 96, d_full = bar0 + 128, d_free = bar0 + 144,
+                 retired = bar0 + 160;
+  const uint32_t ring = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nb = d.n_out / 128, nch = d.n_in / TC_BK;
+  const int per_tile = shared ? 1 : nb;      // items of a row tile; an item is a row tile, or one of its column blocks
+  const int per_item = shared ? nb : 1;      // column blocks of an item
+
+  if (warp == PS_MMA_WARP) {
+    if (lane == 0) {
+      for (int b = 0; b < 4; ++b) { mbar_init(a_ready + 8 * b, 4); mbar_init(a_done + 8 * b, 1); }
+      for (int b = 0; b < 4; ++b) { mbar_init(w_ready + 8 * b, 1); mbar_init(w_done + 8 * b, 1); }
+      for (int b = 0; b < 2; ++b) { mbar_init(d_full + 8 * b, 1); mbar_init(d_free + 8 * b, 8); }
+      mbar_init(retired, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_u32(tmem_slot)), "r"(PS_TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_sync();
+  Walk walk;
+  walk.start(d);
+  int e, rows;
+  int64_t s0;
+
+  if (warp == PS_MMA_WARP) {
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0), ring_u = __shfl_sync(0xffffffffu, ring, 0);
+    bool alive = true;
+    uint32_t g = 0, wu = 0, k = 0;  // A chunks, weight slots, column blocks so far
+    for (int item = blockIdx.x; walk.seek(item / per_tile, e, s0, rows); item += gridDim.x) {
+      for (int j = 0; j < per_item; ++j, ++k) {
+        const uint32_t acc = k & 1, d_tmem = tmem_u + 128u * acc;
+        for (int c = 0; c < nch; ++c, ++wu) {
+          const uint32_t ga = g + c, ab = ga & 3, slot = wu & 3;
+          if (j == 0 && alive) alive = mbar_wait(a_ready + 8 * ab, (ga >> 2) & 1);
+          if (alive) alive = mbar_wait(w_ready + 8 * slot, (wu >> 2) & 1);
+          if (c == 0 && k >= 2 && alive) alive = mbar_wait(d_free + 8 * acc, ((k >> 1) - 1) & 1);
+          alive = __all_sync(0xffffffffu, alive);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (elected) {
+            issue_chunk_mmas<false>(d_tmem, tmem_u + 256 + 64 * ab, ring_u + slot * 2 * TC_TILE_BYTES, 0, c == 0);
+            if (j == per_item - 1) mma_commit(a_done + 8 * ab);
+            mma_commit(w_done + 8 * slot);
+            if (c == nch - 1) mma_commit(d_full + 8 * acc);
+          }
+          __syncwarp();
+        }
+      }
+      g += nch;
+    }
+    drain_mma(retired, elected);
+  } else if (warp == PS_TMA_WARP) {
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    const uint32_t ring_u = __shfl_sync(0xffffffffu, ring, 0);
+    bool alive = true;
+    uint32_t wu = 0;
+    for (int item = blockIdx.x; alive && walk.seek(item / per_tile, e, s0, rows); item += gridDim.x) {
+      for (int j = 0; j < per_item && alive; ++j) {
+        const int row = e * d.n_out + 128 * (shared ? j : item % nb);
+        for (int c = 0; c < nch; ++c, ++wu) {
+          const uint32_t slot = wu & 3;
+          if (wu >= 4) alive = mbar_wait(w_done + 8 * slot, ((wu >> 2) - 1) & 1);
+          alive = __all_sync(0xffffffffu, alive);
+          if (!alive) break;
+          if (elected) {
+            const uint32_t bar = w_ready + 8 * slot, dst = ring_u + slot * 2 * TC_TILE_BYTES;
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(2 * TC_TILE_BYTES) : "memory");
+            tma_load_2d(dst, &maps.hi, bar, c * TC_BK, row);
+            tma_load_2d(dst + TC_TILE_BYTES, &maps.lo, bar, c * TC_BK, row);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    drain_copies(w_ready, 4, wu);
+  } else if (warp >= PS_EPI_WARP0) {
+    // thread = row; epilogue warp e takes columns 64 (e >> 2).. of the accumulator
+    const int quarter = warp & 3, half = (warp - PS_EPI_WARP0) >> 2;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 64);
+    const bool wide = ((reinterpret_cast<uintptr_t>(d.y) | reinterpret_cast<uintptr_t>(d.gate)) & 31u) == 0 && d.ld_y % 8 == 0 && d.ld_gate % 8 == 0;
+    bool alive = true;
+    uint32_t k = 0;
+    for (int item = blockIdx.x; walk.seek(item / per_tile, e, s0, rows); item += gridDim.x) {
+      for (int jj = 0; jj < per_item; ++jj, ++k) {
+        const uint32_t acc = k & 1;
+        const int c0 = 128 * (shared ? jj : item % nb) + 64 * half;
+        const bool valid = quarter * 32 + lane < rows;
+        const int64_t slot = s0 + (valid ? quarter * 32 + lane : 0);
+        const float* const gate = d.gate ? d.gate + slot * d.ld_gate + c0 : nullptr;
+        const float* const bias = d.bias ? d.bias + (int64_t)e * d.n_out + c0 : nullptr;
+        float* const out = d.y + slot * d.ld_y + c0;
+        if (gate) {
+          asm volatile("prefetch.global.L2 [%0];" :: "l"(gate));
+          asm volatile("prefetch.global.L2 [%0];" :: "l"(gate + 32));
+        }
+        if (alive) alive = mbar_wait(d_full + 8 * acc, (k >> 1) & 1);
+        alive = __all_sync(0xffffffffu, alive);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+        for (int cg = 0; cg < 2; ++cg) {
+          uint32_t v[32];
+          MB_TMEM_LD32(lane_base + 128u * acc + 32u * cg, v);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          if (cg == 1) {
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(d_free + 8 * acc);
+          }
+          if (!alive || !valid) continue;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int c = cg * 32 + q * 8;
+            float o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(v[8 * q + i]);
+            if (bias) {
+              const float4 b0 = ld4(bias + c), b1 = ld4(bias + c + 4);
+              add4_to(o, b0);
+              add4_to(o + 4, b1);
+            }
+            if (gate) {
+              const float4 z0 = ld4(gate + c), z1 = ld4(gate + c + 4);
+              silu_grad4_to(o, z0);
+              silu_grad4_to(o + 4, z1);
+            }
+            if (d.out_act) silu_fast_all(o, o);
+            if (wide) st8(out + c, o);
+            else { st4(out + c, make_float4(o[0], o[1], o[2], o[3])); st4(out + c + 4, make_float4(o[4], o[5], o[6], o[7])); }
+          }
+        }
+      }
+    }
+  } else {
+    // producers: lane quarter, K chunks of this warp's parity; thread = row = TMEM lane
+    const int pw = warp - PS_PROD_WARP0, par = pw >> 2, quarter = warp & 3, lr = lane >> 3, lc = lane & 7;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t patch0 = smem_u32(smem + PS_RING_BYTES + pw * (EX_STAGES * 32 * 128));
+    const uint32_t put_even = lr * 128 + ((lc ^ lr) << 4), put_odd = lr * 128 + ((lc ^ (lr | 4)) << 4);
+    Walk ahead = walk;         // of the chunks that are asked for, EX_STAGES - 1 ahead of those that are converted
+    int g_item = blockIdx.x, g_c = 0, g_n = 0;
+    const float* a_ptr[8];
+    int32_t a_row[8];
+    bool more;
+    auto look_up = [&]() {     // the source rows of item g_item, a chunk before they are needed
+      int e_, rows_;
+      int64_t s0_;
+      more = ahead.seek(g_item / per_tile, e_, s0_, rows_);
+      if (!more) return;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = quarter * 32 + lr + 4 * i;
+        const int64_t s = s0_ + (r < rows_ ? r : rows_ - 1);
+        a_row[i] = d.idx ? d.idx[s] : (int32_t)s;
+      }
+    };
+    auto request = [&]() {     // this warp's next chunk into its next patch
+      if (more) {
+        if (g_c == 0) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int64_t r = min(max((int64_t)a_row[i], (int64_t)0), d.n_rows - 1);
+            a_ptr[i] = d.x + r * d.ld_x + par * TC_BK + 4 * lc;
+          }
+        }
+        const uint32_t to = patch0 + (uint32_t)(g_n % EX_STAGES) * (32 * 128);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) copy16(to + ((i & 1) ? put_odd : put_even) + 512u * i, a_ptr[i] + 2 * TC_BK * g_c);
+        ++g_n;
+        if (++g_c == nch / 2) { g_c = 0; g_item += gridDim.x; look_up(); }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    look_up();
+    for (int i = 0; i < EX_STAGES - 1; ++i) request();
+    bool alive = true;
+    uint32_t g = 0;
+    int n = 0;
+    for (int item = blockIdx.x; walk.seek(item / per_tile, e, s0, rows); item += gridDim.x) {
+      for (int c = par; c < nch; c += 2, ++n) {
+        request();  // into the patch read one chunk ago; the __syncwarp that closed that chunk orders the reads
+        asm volatile("cp.async.wait_group %0;" :: "n"(EX_STAGES - 1) : "memory");
+        __syncwarp();
+        const uint32_t patch = patch0 + (uint32_t)(n % EX_STAGES) * (32 * 128), ga = g + c, ab = ga & 3;
+        const uint32_t ta = lane_base + 256 + 64 * ab;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 v = lds4(patch + lane * 128 + (((4 * h + i) ^ (lane & 7)) << 4));
+            x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+          }
+          if (d.in_act) silu_fast_all(x, x);
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float t = to_tf32(x[i]);
+            hi[i] = __float_as_uint(t);
+            lo[i] = __float_as_uint(rest_tf32(x[i], t));
+          }
+          if (h == 0) {
+            if (ga >= 4 && alive) alive = mbar_wait(a_done + 8 * ab, ((ga >> 2) - 1) & 1);  // A buffer ab is free again
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          }
+          MB_TMEM_ST16(ta + 16 * h, hi);
+          MB_TMEM_ST16(ta + 32 + 16 * h, lo);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(a_ready + 8 * ab);
+      }
+      g += nch;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
+
+  if (d.zero_rest) {  // slots behind the last
+    const int64_t used = min(max((int64_t)d.offsets[d.n_experts], (int64_t)0), d.n_slots);
+    for (int64_t s = used + (int64_t)blockIdx.x * (PS_THREADS / 32) + warp; s < d.n_slots; s += (int64_t)gridDim.x * (PS_THREADS / 32))
+      for (int c = 4 * lane; c < d.n_out; c += 128) st4(d.y + s * d.ld_y + c, make_float4(0.f, 0.f, 0.f, 0.f));
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == PS_MMA_WARP) {
+    __syncwarp();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem_base), "r"(PS_TMEM_COLS) : "memory");
+  }
+}
+
+// w [n_out, n_in] of every expert -> tf32 parts hi, lo, and both transposed; 32 x 32 values a block
+__global__ void __launch_bounds__(256) k_experts_split(int n_out, int n_in, int64_t part, const float* __restrict__ w, float* __restrict__ parts) {
+  pdl_sync();
+  __shared__ float t[2][32][33];
+  const int64_t e0 = (int64_t)blockIdx.z * n_out * n_in;
+  const int k0 = blockIdx.x * 32, n0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = ty; i < 32; i += 8) {
+    const int64_t at = e0 + (int64_t)(n0 + i) * n_in + k0 + tx;
+    const float x = w[at], hi = to_tf32(x), lo = rest_tf32(x, hi);
+    parts[at] = hi;
+    parts[part + at] = lo;
+    t[0][i][tx] = hi;
+    t[1][i][tx] = lo;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = ty; i < 32; i += 8) {
+    const int64_t at = e0 + (int64_t)(k0 + i) * n_out + n0 + tx;
+    parts[2 * part + at] = t[0][tx][i];
+    parts[3 * part + at] = t[1][tx][i];
+  }
+}
+
+constexpr int ES_TILE = 64, ES_K = 16, ES_THREADS = 256;
+
+// 64 x 64 of one expert's gradient a block, its slots in order; the first column of blocks sums the bias gradient on the way
+__global__ void __launch_bounds__(ES_THREADS) k_experts_grad_simt(const __grid_constant__ mb_experts d) {
+  pdl_sync();
+  __shared__ float gs[ES_K][ES_TILE + 4], xs[ES_K][ES_TILE + 4];
+  const int e = blockIdx.z, n0 = blockIdx.y * ES_TILE, k0 = blockIdx.x * ES_TILE, tid = threadIdx.x;
+  int64_t from, to;
+  expert_slots(d, e, from, to);
+  const int lr = tid / 16, lc = 4 * (tid % 16), ty = tid / 16, tx = tid % 16;
+  float acc[4][4] = {}, db[4] = {};
+  for (int64_t s0 = from; s0 < to; s0 += ES_K) {
+    const int64_t s = s0 + lr;
+    float4 g = make_float4(0.f, 0.f, 0.f, 0.f), v = g;
+    if (s < to) {
+      g = ld4(d.dy + s * d.ld_dy + n0 + lc);
+      v = ld4(source_row(d, s) + k0 + lc);
+      if (d.in_act) v = make_float4(silu_f(v.x), silu_f(v.y), silu_f(v.z), silu_f(v.w));
+    }
+    __syncthreads();
+    st4(&gs[lr][lc], g);
+    st4(&xs[lr][lc], v);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ES_K; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float gv = gs[k][4 * ty + i];
+        db[i] += gv;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(gv, xs[k][4 * tx + j], acc[i][j]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t n = (int64_t)e * d.n_out + n0 + 4 * ty + i;
+    st4(d.dw + n * d.n_in + k0 + 4 * tx, make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]));
+    if (d.dbias && blockIdx.x == 0 && tx == 0) d.dbias[n] = db[i];
+  }
+}
+

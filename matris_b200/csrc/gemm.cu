@@ -608,6 +608,7 @@ k_gemm_tc(const __grid_constant__ mb_gemm_desc d, const __grid_constant__ TcMaps
 #include "mlp_fused.cuh"
 #include "linear_tma.cuh"
 #include "few_rows.cuh"
+#include "experts.cuh"
 
 // 0: persistent tcgen05 3xBF16 (default), 1: fp32 SIMT, 2: one-tile-per-CTA tcgen05 3xTF32, 3: persistent tcgen05 3xTF32
 static int g_gemm_mode = 0;
@@ -757,6 +758,7 @@ static int device_config(int* n_sm) {
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_gemm_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_SMEM_BYTES));
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_gemm_ps<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PS_SMEM_BYTES));
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_gemm_ps<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PS_SMEM_BYTES));
+    MB_CUDA_CHECK(cudaFuncSetAttribute(k_experts, cudaFuncAttributeMaxDynamicSharedMemorySize, EX_SMEM_BYTES));
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_linear<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM_BYTES));
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_linear<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM_BYTES));
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_mlp<MLP_GATED_FWD, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, ML_SMEM_BYTES));
@@ -1432,5 +1434,59 @@ extern "C" int mb_mlp_bwd_data(const mb_mlp_bwd* g, void* stream_) {
   if (plain) mb::launch(mb::k_mlp<mb::MLP_PLAIN_BWD>, grid, mb::ML_THREADS, mb::ML_SMEM_BYTES, st, a, maps);
   else mb::launch(mb::k_mlp<mb::MLP_GATED_BWD>, grid, mb::ML_THREADS, mb::ML_SMEM_BYTES, st, a, maps);
   MB_LAUNCH_CHECK("k_mlp backward");
+  return MB_OK;
+}
+
+// ------------------------------------------------------------------ experts
+namespace mb {
+static bool aligned_rows(const void* p, int64_t ld, int width) {
+  return p && (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 4 == 0 && ld >= width;
+}
+static bool experts_valid(const mb_experts* d) {
+  return d && d->n_slots >= 0 && d->n_slots <= INT32_MAX && d->n_rows >= 0 && d->n_experts >= 1 && d->n_experts <= EX_MAX_EXPERTS &&
+         d->n_in >= 128 && d->n_in <= EX_MAX_WIDTH && d->n_in % 128 == 0 && d->n_out >= 128 && d->n_out <= EX_MAX_WIDTH && d->n_out % 128 == 0 &&
+         d->offsets && (d->n_slots == 0 || (aligned_rows(d->x, d->ld_x, d->n_in) && (d->idx ? d->n_rows >= 1 : d->n_rows >= d->n_slots)));
+}
+
+}  // namespace mb
+
+extern "C" int mb_experts_split(int32_t n_experts, int32_t n_out, int32_t n_in, const float* w, float* parts, void* stream) {
+  if (n_experts < 1 || n_experts > mb::EX_MAX_EXPERTS || n_out < 128 || n_out > mb::EX_MAX_WIDTH || n_out % 128 || n_in < 128 || n_in > mb::EX_MAX_WIDTH ||
+      n_in % 128 || !w || !parts || (reinterpret_cast<uintptr_t>(parts) & 15u))
+    return MB_ERR_INVALID;
+  mb::launch(mb::k_experts_split, dim3((unsigned)(n_in / 32), (unsigned)(n_out / 32), (unsigned)n_experts), 256, 0, (cudaStream_t)stream, n_out, n_in,
+         (int64_t)n_experts * n_out * n_in, w, parts);
+  MB_LAUNCH_CHECK("k_experts_split");
+  return MB_OK;
+}
+
+extern "C" int mb_experts_linear(const mb_experts* d, void* stream) {
+  if (!mb::experts_valid(d) || !mb::aligned_rows(d->w_hi, d->n_in, d->n_in) || !mb::aligned_rows(d->w_lo, d->n_in, d->n_in)) return MB_ERR_INVALID;
+  if (d->bias && !mb::aligned_rows(d->bias, d->n_out, d->n_out)) return MB_ERR_INVALID;
+  if (d->n_slots == 0) return MB_OK;
+  if (!mb::aligned_rows(d->y, d->ld_y, d->n_out) || (d->gate && !mb::aligned_rows(d->gate, d->ld_gate, d->n_out))) return MB_ERR_INVALID;
+  int n_sm = 0, rc = mb::device_config(&n_sm);
+  if (rc) return rc;
+  mb::ExMaps maps;
+  const int rows = d->n_experts * d->n_out;
+  if ((rc = mb::weight_map(d->w_hi, d->n_in, d->n_in, &maps.hi, rows)) || (rc = mb::weight_map(d->w_lo, d->n_in, d->n_in, &maps.lo, rows))) return rc;
+  const int shared = d->n_in == 128 ? 1 : 0;
+  const int64_t items = ((d->n_slots + 127) / 128 + d->n_experts) * (shared ? 1 : d->n_out / 128);
+  mb::launch(mb::k_experts, (unsigned)(items < n_sm ? items : n_sm), mb::PS_THREADS, mb::EX_SMEM_BYTES, (cudaStream_t)stream, *d, maps, shared);
+  MB_LAUNCH_CHECK("k_experts");
+  return MB_OK;
+}
+
+extern "C" size_t mb_experts_grad_scratch(int64_t n_slots, int32_t n_experts, int32_t n_in, int32_t n_out) {
+  (void)n_slots; (void)n_experts; (void)n_in; (void)n_out;
+  return 0;
+}
+
+extern "C" int mb_experts_grad_w(const mb_experts* d, void* stream) {
+  if (!mb::experts_valid(d) || !mb::aligned_rows(d->dw, d->n_in, d->n_in)) return MB_ERR_INVALID;
+  if (d->n_slots > 0 && !mb::aligned_rows(d->dy, d->ld_dy, d->n_out)) return MB_ERR_INVALID;
+  const dim3 grid((unsigned)(d->n_in / mb::ES_TILE), (unsigned)(d->n_out / mb::ES_TILE), (unsigned)d->n_experts);
+  mb::launch(mb::k_experts_grad_simt, grid, mb::ES_THREADS, 0, (cudaStream_t)stream, *d);
+  MB_LAUNCH_CHECK("k_experts_grad_simt");
   return MB_OK;
 }

@@ -660,9 +660,10 @@ def route_bwd(logits, route: Route, dweights=None, dloss=None):
 
 
 class ExpertWeights:
-    """Weights [experts, n_out, n_in] of the experts' dense layers, laid out once for ``experts_linear`` in both directions."""
+    """Weights [experts, n_out, n_in] of the experts' dense layers, laid out once for ``experts_linear`` in both directions:
+    two tf32 parts each, w = hi + lo to 2^-23, 16 bytes a weight.  It copies: a later change of ``w`` does not reach it."""
 
-    __slots__ = ("w", "wt")
+    __slots__ = ("shape", "parts")
 
     def __init__(self, w: torch.Tensor):
         w = _take(w.detach(), "weights", torch.float32, (None, None, None), dense=False).contiguous()
@@ -670,7 +671,8 @@ class ExpertWeights:
             raise NotImplementedError(f"1 to 1024 experts, got {w.shape[0]}")
         _expert_widths(w.shape[2], w.shape[1])
         _here(weights=w)
-        self.w, self.wt = w, w.transpose(1, 2).contiguous()
+        self.shape, self.parts = tuple(w.shape), new(4, w.numel(), w)
+        call("mb_experts_split", *self.shape, ptr(w), ptr(self.parts), _stream())
 
 
 def _expert_widths(n_in, n_out):
@@ -706,8 +708,10 @@ def experts_linear(x, weights, offsets, bias=None, idx=None, in_act=0, out_act=0
     Slots behind the last are zero in a returned tensor and left alone in a given ``out``."""
     if not isinstance(weights, ExpertWeights):
         weights = ExpertWeights(weights)
-    w = weights.wt if transposed else weights.w
-    n_experts, n_out, n_in = w.shape
+    n_experts, n_out, n_in = weights.shape
+    w_hi = ptr(weights.parts) + (8 * weights.parts.shape[1] if transposed else 0)
+    if transposed:
+        n_out, n_in = n_in, n_out
     d = _experts_desc(x, offsets, idx, n_in, n_out, in_act)
     if d.n_experts != n_experts:
         raise ValueError(f"offsets: [{n_experts + 1}] is wanted, got {tuple(offsets.shape)}")
@@ -720,9 +724,10 @@ def experts_linear(x, weights, offsets, bias=None, idx=None, in_act=0, out_act=0
         d.gate, d.ld_gate = ptr(gate), _aligned_rows(gate, "gate")
     if out is not None:
         _take(out, "out", torch.float32, (d.n_slots, n_out), dense=False)
-    _here(x=x, weights=w, offsets=offsets, bias=bias, idx=idx, gate=gate, out=out)
+    _here(x=x, weights=weights.parts, offsets=offsets, bias=bias, idx=idx, gate=gate, out=out)
     y = new(d.n_slots, n_out, x) if out is None else out
-    d.w, d.bias, d.out_act, d.zero_rest = ptr(w), ptr(bias), out_act, int(out is None)
+    d.w_hi, d.w_lo = w_hi, w_hi + 4 * weights.parts.shape[1]
+    d.bias, d.out_act, d.zero_rest = ptr(bias), out_act, int(out is None)
     d.y, d.ld_y = ptr(y), _aligned_rows(y, "out")
     call("mb_experts_linear", C.byref(d), _stream())
     return y
