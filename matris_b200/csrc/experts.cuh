@@ -29,8 +29,8 @@ __device__ __forceinline__ const float* source_row(const mb_experts& d, int64_t 
 // tile of its own and its rows are gathered again, from L2.
 struct alignas(64) ExMaps { CUtensorMap hi, lo; };
 
-// Tiles of 128 slots in order of expert; all lanes of a warp call it together
-struct Walk {
+// Tiles of 2^SHIFT slots in order of expert; all lanes of a warp call it together
+template <int SHIFT> struct Walk {
   const mb_experts* d;
   int base, before, total;   // first expert held (lane l: base + l), tiles ahead of it, tiles of the 32
   int64_t from, to;
@@ -39,7 +39,7 @@ struct Walk {
     const int lane = threadIdx.x & 31, e = base + lane;
     from = to = 0;
     if (e < d->n_experts) expert_slots(*d, e, from, to);
-    upto = (int)((to - from + 127) >> 7);
+    upto = (int)((to - from + (1 << SHIFT) - 1) >> SHIFT);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, upto, o);
@@ -48,8 +48,9 @@ struct Walk {
     total = __shfl_sync(0xffffffffu, upto, 31);
   }
   __device__ __forceinline__ void start(const mb_experts& args) { d = &args; base = before = 0; load(); }
-  // tile t (never less than the last one asked for): its expert, first slot and number of slots; false: there are no more
-  __device__ __forceinline__ bool seek(int t, int& e, int64_t& s0, int& rows) {
+  // tile t (never less than the last one asked for): its expert, first slot, the expert's slots from there on and whether it is the
+  // expert's first tile; false: there are no more
+  __device__ __forceinline__ bool seek(int t, int& e, int64_t& s0, int64_t& left, bool& first) {
     while (t - before >= total) {
       before += total;
       base += 32;
@@ -57,12 +58,27 @@ struct Walk {
       load();
     }
     const int at = __popc(__ballot_sync(0xffffffffu, t - before >= upto));
-    const int ahead = __shfl_sync(0xffffffffu, upto, at > 0 ? at - 1 : 0), first = at > 0 ? ahead : 0;
+    const int ahead = __shfl_sync(0xffffffffu, upto, at > 0 ? at - 1 : 0), nth = t - before - (at > 0 ? ahead : 0);
     e = base + at;
-    s0 = __shfl_sync(0xffffffffu, from, at) + (int64_t)(t - before - first) * 128;
-    const int64_t left = __shfl_sync(0xffffffffu, to, at) - s0;
-    rows = left < 128 ? (int)left : 128;
+    s0 = __shfl_sync(0xffffffffu, from, at) + ((int64_t)nth << SHIFT);
+    left = __shfl_sync(0xffffffffu, to, at) - s0;
+    first = nth == 0;
     return true;
+  }
+  __device__ __forceinline__ bool seek(int t, int& e, int64_t& s0, int& rows) {
+    int64_t left;
+    bool first;
+    if (!seek(t, e, s0, left, first)) return false;
+    rows = left < (1 << SHIFT) ? (int)left : 1 << SHIFT;
+    return true;
+  }
+  // all tiles; the walk is at the start again
+  __device__ __forceinline__ int64_t count() {
+    int64_t n = 0;
+    for (int b = 0; b < d->n_experts; b += 32) { base = b; load(); n += total; }
+    base = before = 0;
+    load();
+    return n;
   }
 };
 
@@ -111,7 +127,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *tmem_slot;
   pdl_sync();
-  Walk walk;
+  Walk<7> walk;
   walk.start(d);
   int e, rows;
   int64_t s0;
@@ -232,7 +248,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t patch0 = smem_u32(smem + PS_RING_BYTES + pw * (EX_STAGES * 32 * 128));
     const uint32_t put_even = lr * 128 + ((lc ^ lr) << 4), put_odd = lr * 128 + ((lc ^ (lr | 4)) << 4);
-    Walk ahead = walk;         // of the chunks that are asked for, EX_STAGES - 1 ahead of those that are converted
+    Walk<7> ahead = walk;         // of the chunks that are asked for, EX_STAGES - 1 ahead of those that are converted
     int g_item = blockIdx.x, g_c = 0, g_n = 0;
     const float* a_ptr[8];
     int32_t a_row[8];
@@ -349,44 +365,313 @@ __global__ void __launch_bounds__(256) k_experts_split(int n_out, int n_in, int6
   }
 }
 
-constexpr int ES_TILE = 64, ES_K = 16, ES_THREADS = 256;
+// ------------------------------------------------------------------ weight gradient
+// dW_e = sum over the slots of e of dy[s]^T f(x[idx[s]]): the contraction runs over rows, so both operands have to be turned.  A
+// thread that holds a COLUMN does that for free: lanes of a warp read 32 neighbouring values of a row, row after row, and own one
+// column each.  dy columns (lane = row of dW) go to tensor memory as the A operand, x columns to shared memory as the K-major B
+// operand, in chunks of 32 rows, both as two tf32 parts (k_experts has the arithmetic).
+//
+// Work is cut by rows, not by experts: the chunks of all experts, numbered through, are shared out evenly over the CTAs of a 128 x 128
+// block of dW (a share may begin and end inside an expert), so that one expert with most rows costs no more than even ones.  A run of
+// chunks that holds all of an expert goes straight to dW; the others, two a share at the most, are left as partial sums and joined in
+// order by k_experts_grad_join.
+//
+// The tensor cores cut each sum they accumulate to float32 instead of rounding it, always towards zero: after n of them a sum is
+// short by up to n 2^-23.  So a run is accumulated there for EG_FLUSH chunks only and added up in float32 registers of the epilogue
+// warps, rounded to nearest.
+//
+// Roles: warp 0 issues the products, warp 1 asks L2 for the rows four chunks ahead, warps 2 - 5 hold dy's columns, 6 - 9 x's, 10 - 17
+// the sums.
+#define MB_TMEM_LD16(taddr, v)                                                                                   \
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "                                                         \
+               "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"                  \
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), \
+                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),        \
+                 "=r"(v[15]) : "r"(taddr) : "memory")
+constexpr int EG_FLUSH = 4;
+constexpr int EG_AHEAD = 4;
+constexpr int EG_BUFS = 4;
+constexpr int EG_BAR_OFF = EG_BUFS * 2 * TC_TILE_BYTES;
+constexpr int EG_SMEM_BYTES = EG_BAR_OFF + 256;
 
-// 64 x 64 of one expert's gradient a block, its slots in order; the first column of blocks sums the bias gradient on the way
-__global__ void __launch_bounds__(ES_THREADS) k_experts_grad_simt(const __grid_constant__ mb_experts d) {
-  pdl_sync();
-  __shared__ float gs[ES_K][ES_TILE + 4], xs[ES_K][ES_TILE + 4];
-  const int e = blockIdx.z, n0 = blockIdx.y * ES_TILE, k0 = blockIdx.x * ES_TILE, tid = threadIdx.x;
-  int64_t from, to;
-  expert_slots(d, e, from, to);
-  const int lr = tid / 16, lc = 4 * (tid % 16), ty = tid / 16, tx = tid % 16;
-  float acc[4][4] = {}, db[4] = {};
-  for (int64_t s0 = from; s0 < to; s0 += ES_K) {
-    const int64_t s = s0 + lr;
-    float4 g = make_float4(0.f, 0.f, 0.f, 0.f), v = g;
-    if (s < to) {
-      g = ld4(d.dy + s * d.ld_dy + n0 + lc);
-      v = ld4(source_row(d, s) + k0 + lc);
-      if (d.in_act) v = make_float4(silu_f(v.x), silu_f(v.y), silu_f(v.z), silu_f(v.w));
-    }
-    __syncthreads();
-    st4(&gs[lr][lc], g);
-    st4(&xs[lr][lc], v);
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < ES_K; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float gv = gs[k][4 * ty + i];
-        db[i] += gv;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(gv, xs[k][4 * tx + j], acc[i][j]);
-      }
+struct GradShare {  // chunks [lo, hi) of share c of n
+  int64_t all, lo, hi;
+  __device__ __forceinline__ GradShare(int64_t all_, int c, int n) : all(all_), lo(all_ * c / n), hi(all_ * (c + 1) / n) {}
+  static __device__ __forceinline__ int of(int64_t chunk, int64_t all, int n) { return (int)(((chunk + 1) * n - 1) / all); }
+};
+
+__global__ void __launch_bounds__(PS_THREADS, 1)
+k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* const part, float* const part_bias) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + EG_BAR_OFF);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + EG_BAR_OFF + 240);
+  volatile uint32_t* const issued = reinterpret_cast<volatile uint32_t*>(smem + EG_BAR_OFF + 248);  // chunks whose products are under way
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicOr(&g_gemm_status, 2);
+    return;
   }
+  // ready[4] (8 column warps) done[4] | d_full[2] d_free[2] (8 epilogue warps) | retired
+  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t ready = bar0, done = bar0 + 32, d_full = bar0 + 64, d_free = bar0 + 80, retired = bar0 + 96;
+  const uint32_t tiles = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nk = d.n_in / 128, nb = nk * (d.n_out / 128);
+  const int c = blockIdx.x / nb, n0 = 128 * (blockIdx.x % nb / nk), k0 = 128 * (blockIdx.x % nk);
+
+  if (warp == PS_MMA_WARP) {
+    if (lane == 0) {
+      *issued = 0;
+      for (int b = 0; b < 4; ++b) { mbar_init(ready + 8 * b, 8); mbar_init(done + 8 * b, 1); }
+      for (int b = 0; b < 2; ++b) { mbar_init(d_full + 8 * b, 1); mbar_init(d_free + 8 * b, 8); }
+      mbar_init(retired, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_u32(tmem_slot)), "r"(PS_TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_sync();
+  Walk<5> walk;
+  walk.start(d);
+  const GradShare share(walk.count(), c, n_share);
+  int e;
+  int64_t s0, left;
+  bool first;
+  bool alive = true;
+
+  if (warp == PS_MMA_WARP) {
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0), tiles_u = __shfl_sync(0xffffffffu, tiles, 0);
+    uint32_t g = 0, k = 0, in_acc = 0;
+    for (int64_t t = share.lo; t < share.hi && walk.seek((int)t, e, s0, left, first); ++t, ++g) {
+      const uint32_t b = g & 3, acc = k & 1;
+      if (alive) alive = mbar_wait(ready + 8 * b, (g >> 2) & 1);
+      if (in_acc == 0 && k >= 2 && alive) alive = mbar_wait(d_free + 8 * acc, ((k >> 1) - 1) & 1);
+      alive = __all_sync(0xffffffffu, alive);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const bool flush = in_acc == EG_FLUSH - 1 || left <= 32 || t + 1 == share.hi;
+      if (elected) {
+        issue_chunk_mmas<false>(tmem_u + 128u * acc, tmem_u + 256 + 64 * b, tiles_u + b * 2 * TC_TILE_BYTES, 0, in_acc == 0);
+        mma_commit(done + 8 * b);
+        if (flush) mma_commit(d_full + 8 * acc);
+      }
+      __syncwarp();
+      if (lane == 0) *issued = g + 1;
+      ++in_acc;
+      if (flush) { in_acc = 0; ++k; }
+    }
+    drain_mma(retired, elected);
+  } else if (warp == PS_TMA_WARP) {
+    // lane = row of a chunk: four lines of dy, four of x.  A hint only: it waits for the products (a bounded number of naps) but nothing
+    // waits for it
+    for (int64_t t = share.lo; t < share.hi && walk.seek((int)t, e, s0, left, first); ++t) {
+      for (int naps = 0; naps < 1 << 16 && t - share.lo > (int64_t)*issued + EG_AHEAD; ++naps) __nanosleep(100);
+      if (lane < left) {
+        const float* const g = d.dy + (s0 + lane) * d.ld_dy + n0;
+        const float* const x = source_row(d, s0 + lane) + k0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t n = (int64_t)e * d.n_out + n0 + 4 * ty + i;
-    st4(d.dw + n * d.n_in + k0 + 4 * tx, make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]));
-    if (d.dbias && blockIdx.x == 0 && tx == 0) d.dbias[n] = db[i];
+        for (int i = 0; i < 4; ++i) {
+          asm volatile("prefetch.global.L2 [%0];" :: "l"(g + 32 * i));
+          asm volatile("prefetch.global.L2 [%0];" :: "l"(x + 32 * i));
+        }
+      }
+    }
+  } else if (warp >= PS_EPI_WARP0) {
+    // thread = row of the block, 64 of its columns; sums of a run in registers
+    const int quarter = warp & 3, half = (warp - PS_EPI_WARP0) >> 2;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 64);
+    const int64_t at = (int64_t)(n0 + quarter * 32 + lane) * d.n_in + k0 + 64 * half, whole = (int64_t)d.n_out * d.n_in;
+    f2 sum[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) sum[i] = two(0.f, 0.f);
+    uint32_t k = 0, in_acc = 0;
+    bool fresh = true, from_start = false;
+    for (int64_t t = share.lo; t < share.hi && walk.seek((int)t, e, s0, left, first); ++t) {
+      if (fresh) { from_start = first; fresh = false; }
+      const bool end = left <= 32 || t + 1 == share.hi;
+      if (++in_acc < EG_FLUSH && !end) continue;
+      in_acc = 0;
+      const uint32_t acc = k & 1;
+      if (alive) alive = mbar_wait(d_full + 8 * acc, (k >> 1) & 1);
+      alive = __all_sync(0xffffffffu, alive);
+      ++k;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+      for (int cg = 0; cg < 4; ++cg) {
+        uint32_t v[16];
+        MB_TMEM_LD16(lane_base + 128u * acc + 16u * cg, v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[8 * cg + i] = sum[8 * cg + i] + two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(d_free + 8 * acc);
+      if (end) {
+        float* const out = (from_start && left <= 32 ? d.dw + e * whole : part + (2 * c + (from_start ? 1 : 0)) * whole) + at;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float o[4];
+          apart(sum[2 * i], o[0], o[1]);
+          apart(sum[2 * i + 1], o[2], o[3]);
+          if (alive) st4(out + 4 * i, make_float4(o[0], o[1], o[2], o[3]));
+          sum[2 * i] = sum[2 * i + 1] = two(0.f, 0.f);
+        }
+        fresh = true;
+      }
+    }
+  } else {
+    // columns: warps 2 - 5 dy (A, tensor memory), 6 - 9 x (B, shared memory), 32 columns each
+    const bool is_x = warp >= PS_PROD_WARP0 + 4;
+    const int quarter = warp & 3, col = 32 * quarter + lane;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + 256;
+    float v[32];               // this lane's column of a chunk; a half is asked for as soon as it has been used
+    Walk<5> ahead = walk;
+    int64_t t_ask = share.lo, next_ld = is_x ? d.ld_x : d.ld_dy;
+    int rows = 0, row = 0;     // of the chunk asked for; x: lane's source row
+    const float* next = nullptr;
+    auto look_up = [&]() {
+      int e_;
+      int64_t s_;
+      rows = 0;
+      if (t_ask >= share.hi || !ahead.seek((int)t_ask++, e_, s_, rows)) return;
+      if (is_x) {
+        row = lane < rows ? (d.idx ? d.idx[s_ + lane] : (int32_t)(s_ + lane)) : 0;
+        row = (int32_t)min(max((int64_t)row, (int64_t)0), d.n_rows - 1);
+        next = d.x + k0 + col;
+      } else {
+        row = lane;
+        next = d.dy + s_ * d.ld_dy + n0 + col;
+      }
+    };
+    auto ask = [&](int h) {
+#pragma unroll
+      for (int i = 16 * h; i < 16 * h + 16; ++i) {
+        const int64_t r = is_x ? __shfl_sync(0xffffffffu, row, i) : i;
+        v[i] = i < rows ? next[r * next_ld] : 0.f;
+      }
+    };
+    look_up();
+    ask(0);
+    ask(1);
+    uint32_t g = 0;
+    float bias = 0.f;
+    bool fresh = true, from_start = false;
+    for (int64_t t = share.lo; t < share.hi && walk.seek((int)t, e, s0, left, first); ++t, ++g) {
+      const uint32_t b = g & 3;
+      look_up();
+      if (g >= 4 && alive) alive = mbar_wait(done + 8 * b, ((g >> 2) - 1) & 1);
+      alive = __all_sync(0xffffffffu, alive);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t line = tiles + b * 2 * TC_TILE_BYTES + col * 128;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t hi[16], lo[16];
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = v[16 * h + i];
+        if (is_x && d.in_act) silu_fast_all(x, x);
+        if (!is_x) {
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) sum += (x[i] + x[i + 1]) + (x[i + 2] + x[i + 3]);
+          bias += sum;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float f = to_tf32(x[i]);
+          hi[i] = __float_as_uint(f);
+          lo[i] = __float_as_uint(rest_tf32(x[i], f));
+        }
+        if (is_x) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t to = line + (((4 * h + i) ^ (col & 7)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                         :: "r"(to), "r"(hi[4 * i]), "r"(hi[4 * i + 1]), "r"(hi[4 * i + 2]), "r"(hi[4 * i + 3]) : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                         :: "r"(to + TC_TILE_BYTES), "r"(lo[4 * i]), "r"(lo[4 * i + 1]), "r"(lo[4 * i + 2]), "r"(lo[4 * i + 3]) : "memory");
+          }
+        } else {
+          MB_TMEM_ST16(lane_base + 64 * b + 16 * h, hi);
+          MB_TMEM_ST16(lane_base + 64 * b + 32 + 16 * h, lo);
+        }
+        ask(h);
+      }
+      if (is_x) {
+        to_async_proxy();
+      } else {
+        if (fresh) { from_start = first; fresh = false; }
+        if (left <= 32 || t + 1 == share.hi) {
+          if (part_bias && k0 == 0) {
+            float* const out = from_start && left <= 32 ? d.dbias + (int64_t)e * d.n_out : part_bias + (int64_t)(2 * c + (from_start ? 1 : 0)) * d.n_out;
+            out[n0 + col] = bias;
+          }
+          bias = 0.f;
+          fresh = true;
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ready + 8 * b);
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == PS_MMA_WARP) {
+    __syncwarp();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem_base), "r"(PS_TMEM_COLS) : "memory");
   }
 }
 
+// The partial sums of experts whose slots lie in more than one share, in order of share; zeros for experts without slots.
+// blockIdx.y = expert; the bias gradient is the last n_out values of an expert's part
+__global__ void __launch_bounds__(256) k_experts_grad_join(const __grid_constant__ mb_experts d, const int n_share, const float* __restrict__ part,
+                                                           const float* __restrict__ part_bias) {
+  pdl_sync();
+  const int e = blockIdx.y;
+  Walk<5> walk;
+  walk.start(d);
+  int64_t before = 0, mine = 0, all = 0;
+  for (int b = 0; b < d.n_experts; b += 32) {
+    walk.base = b;
+    walk.load();
+    if (e >= b && e < b + 32) {
+      const int upto = __shfl_sync(0xffffffffu, walk.upto, e - b), ahead = __shfl_sync(0xffffffffu, walk.upto, e > b ? e - b - 1 : 0);
+      before = all + (e > b ? ahead : 0);
+      mine = all + upto - before;
+    }
+    all += walk.total;
+  }
+  int c0 = 0, c1 = 0;
+  if (mine > 0) {
+    c0 = GradShare::of(before, all, n_share);
+    c1 = GradShare::of(before + mine - 1, all, n_share);
+    if (c0 == c1) return;  // in dW already
+  }
+  const int64_t whole = (int64_t)d.n_out * d.n_in;
+  const int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  const bool is_bias = i >= whole;
+  if (is_bias && (!d.dbias || i >= whole + d.n_out)) return;
+  const int64_t stride = is_bias ? d.n_out : whole, at = is_bias ? i - whole : i;
+  const float* const from = is_bias ? part_bias : part;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (mine > 0) {
+    s = ld4(from + (2 * (int64_t)c0 + 1) * stride + at);
+    for (int c = c0 + 1; c <= c1; ++c) {
+      const GradShare share(all, c, n_share);
+      if (share.lo < share.hi) s = add4(s, ld4(from + 2 * (int64_t)c * stride + at));
+    }
+  }
+  st4((is_bias ? d.dbias : d.dw) + e * stride + at, s);
+}

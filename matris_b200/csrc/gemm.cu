@@ -758,6 +758,7 @@ static int device_config(int* n_sm) {
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_gemm_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_SMEM_BYTES));
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_gemm_ps<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PS_SMEM_BYTES));
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_gemm_ps<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PS_SMEM_BYTES));
+    MB_CUDA_CHECK(cudaFuncSetAttribute(k_experts_grad, cudaFuncAttributeMaxDynamicSharedMemorySize, EG_SMEM_BYTES));
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_experts, cudaFuncAttributeMaxDynamicSharedMemorySize, EX_SMEM_BYTES));
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_linear<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM_BYTES));
     MB_CUDA_CHECK(cudaFuncSetAttribute(k_linear<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM_BYTES));
@@ -1477,16 +1478,35 @@ extern "C" int mb_experts_linear(const mb_experts* d, void* stream) {
   return MB_OK;
 }
 
+// Shares of the rows: one CTA a multiprocessor over all blocks of dW, and no more than there can be chunks of 32 rows
+static int experts_shares(int64_t n_slots, int n_experts, int n_in, int n_out, int n_sm) {
+  const int nb = (n_in / 128) * (n_out / 128);
+  const int64_t chunks = (n_slots + 31) / 32 + n_experts, fit = n_sm / nb > 0 ? n_sm / nb : 1;
+  return (int)(chunks < fit ? chunks : fit);
+}
+
 extern "C" size_t mb_experts_grad_scratch(int64_t n_slots, int32_t n_experts, int32_t n_in, int32_t n_out) {
-  (void)n_slots; (void)n_experts; (void)n_in; (void)n_out;
-  return 0;
+  int n_sm = 0;
+  if (n_slots < 0 || n_experts < 1 || n_in < 128 || n_out < 128 || mb::sm_count(&n_sm) != MB_OK) return 0;
+  return 2 * (size_t)experts_shares(n_slots, n_experts, n_in, n_out, n_sm) * (size_t)n_out * (size_t)(n_in + 1) * sizeof(float);
 }
 
 extern "C" int mb_experts_grad_w(const mb_experts* d, void* stream) {
   if (!mb::experts_valid(d) || !mb::aligned_rows(d->dw, d->n_in, d->n_in)) return MB_ERR_INVALID;
-  if (d->n_slots > 0 && !mb::aligned_rows(d->dy, d->ld_dy, d->n_out)) return MB_ERR_INVALID;
-  const dim3 grid((unsigned)(d->n_in / mb::ES_TILE), (unsigned)(d->n_out / mb::ES_TILE), (unsigned)d->n_experts);
-  mb::launch(mb::k_experts_grad_simt, grid, mb::ES_THREADS, 0, (cudaStream_t)stream, *d);
-  MB_LAUNCH_CHECK("k_experts_grad_simt");
+  if (d->dbias && (reinterpret_cast<uintptr_t>(d->dbias) & 15u)) return MB_ERR_INVALID;
+  if (d->n_slots > 0 && (!mb::aligned_rows(d->dy, d->ld_dy, d->n_out) || !mb::aligned_rows(d->scratch, 4, 4))) return MB_ERR_INVALID;
+  int n_sm = 0, rc = mb::device_config(&n_sm);
+  if (rc) return rc;
+  const int n_share = experts_shares(d->n_slots, d->n_experts, d->n_in, d->n_out, n_sm);
+  const int64_t whole = (int64_t)d->n_out * d->n_in;
+  float* const part = static_cast<float*>(d->scratch);
+  float* const part_bias = d->dbias && part ? part + 2 * n_share * whole : nullptr;
+  if (d->n_slots > 0) {
+    const unsigned grid = (unsigned)(n_share * (d->n_in / 128) * (d->n_out / 128));
+    mb::launch(mb::k_experts_grad, grid, mb::PS_THREADS, mb::EG_SMEM_BYTES, (cudaStream_t)stream, *d, n_share, part, part_bias);
+  }
+  mb::launch(mb::k_experts_grad_join, dim3((unsigned)mb::cdiv(whole + d->n_out, 1024), (unsigned)d->n_experts), 256, 0, (cudaStream_t)stream, *d, n_share,
+             part, part_bias);
+  MB_LAUNCH_CHECK("k_experts_grad");
   return MB_OK;
 }
