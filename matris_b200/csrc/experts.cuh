@@ -21,8 +21,8 @@ __device__ __forceinline__ const float* source_row(const mb_experts& d, int64_t 
 // through idx, its weights are rows e n_out + 128 j .. of one tensor map over all experts' weights.  Rows behind the expert's last slot
 // repeat it and are not stored: the next expert's rows belong to another tile.
 //
-// Operands are split into two tf32 parts, both rounded to nearest: x = hi + lo to 2^-23, and the three products kept drop lo lo,
-// at most 2^-22 of |x w| and of either sign: the float32 rounding of the sums is as large.  (Two bf16 parts, as the other dense
+// Operands are split into two tf32 parts, hi rounded to nearest: x = hi + lo to 2^-22, and the three products kept drop lo lo, at
+// most 2^-24 of |x w| and of either sign: the float32 rounding of the sums is as large.  (Two bf16 parts, as the other dense
 // layers have, are twice as fast and good to 2^-17: of no use here, where memory bounds the call either way.)
 //
 // shared (K = 128): the four A buffers hold the whole row tile, converted once for all its column blocks.  Otherwise a column block is a
@@ -88,7 +88,12 @@ constexpr int EX_BAR_OFF = PS_RING_BYTES + EX_PATCH_BYTES;
 constexpr int EX_SMEM_BYTES = EX_BAR_OFF + 256;
 static_assert(EX_SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
 
-__device__ __forceinline__ float rest_tf32(float x, float hi) { return to_tf32(x - hi); }
+// x = hi + lo, hi rounded to 11 significant bits by integer arithmetic (the conversion instruction runs at an eighth of the rate: two of
+// them a value took 512 cycles of the 768 that a chunk's products need).  The tensor cores read lo's leading 11 bits, of |lo| <= 2^-12 |x|.
+__device__ __forceinline__ void split_tf32_even(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
 
 __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant__ mb_experts d, const __grid_constant__ ExMaps maps, const int shared) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -248,81 +253,70 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t patch0 = smem_u32(smem + PS_RING_BYTES + pw * (EX_STAGES * 32 * 128));
     const uint32_t put_even = lr * 128 + ((lc ^ lr) << 4), put_odd = lr * 128 + ((lc ^ (lr | 4)) << 4);
-    Walk<7> ahead = walk;         // of the chunks that are asked for, EX_STAGES - 1 ahead of those that are converted
-    int g_item = blockIdx.x, g_c = 0, g_n = 0;
-    const float* a_ptr[8];
-    int32_t a_row[8];
+    // The walk is that of the chunks asked for, EX_STAGES - 1 ahead of those converted; the rows of an item are looked up a chunk before
+    // they are needed.  This warp's n-th chunk is chunk 2 n + par of the CTA.
+    int item = blockIdx.x, g_c = 0, asked = 0;
+    int32_t a_row[8], next_row[8];
     bool more;
-    auto look_up = [&]() {     // the source rows of item g_item, a chunk before they are needed
-      int e_, rows_;
-      int64_t s0_;
-      more = ahead.seek(g_item / per_tile, e_, s0_, rows_);
+    const float* const x = d.x + par * TC_BK + 4 * lc;
+    auto look_up = [&]() {
+      more = walk.seek(item / per_tile, e, s0, rows);
       if (!more) return;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = quarter * 32 + lr + 4 * i;
-        const int64_t s = s0_ + (r < rows_ ? r : rows_ - 1);
-        a_row[i] = d.idx ? d.idx[s] : (int32_t)s;
+        const int64_t s = s0 + (r < rows ? r : rows - 1);
+        next_row[i] = d.idx ? d.idx[s] : (int32_t)s;
       }
     };
     auto request = [&]() {     // this warp's next chunk into its next patch
       if (more) {
         if (g_c == 0) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int64_t r = min(max((int64_t)a_row[i], (int64_t)0), d.n_rows - 1);
-            a_ptr[i] = d.x + r * d.ld_x + par * TC_BK + 4 * lc;
-          }
+          for (int i = 0; i < 8; ++i) a_row[i] = (int32_t)min(max((int64_t)next_row[i], (int64_t)0), d.n_rows - 1);
         }
-        const uint32_t to = patch0 + (uint32_t)(g_n % EX_STAGES) * (32 * 128);
+        const uint32_t to = patch0 + (uint32_t)(asked % EX_STAGES) * (32 * 128);
+        const float* const from = x + 2 * TC_BK * g_c;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) copy16(to + ((i & 1) ? put_odd : put_even) + 512u * i, a_ptr[i] + 2 * TC_BK * g_c);
-        ++g_n;
-        if (++g_c == nch / 2) { g_c = 0; g_item += gridDim.x; look_up(); }
+        for (int i = 0; i < 8; ++i) copy16(to + ((i & 1) ? put_odd : put_even) + 512u * i, from + (int64_t)a_row[i] * (int)d.ld_x);
+        ++asked;
+        if (++g_c == nch / 2) { g_c = 0; item += gridDim.x; look_up(); }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     look_up();
     for (int i = 0; i < EX_STAGES - 1; ++i) request();
     bool alive = true;
-    uint32_t g = 0;
-    int n = 0;
-    for (int item = blockIdx.x; walk.seek(item / per_tile, e, s0, rows); item += gridDim.x) {
-      for (int c = par; c < nch; c += 2, ++n) {
-        request();  // into the patch read one chunk ago; the __syncwarp that closed that chunk orders the reads
-        asm volatile("cp.async.wait_group %0;" :: "n"(EX_STAGES - 1) : "memory");
-        __syncwarp();
-        const uint32_t patch = patch0 + (uint32_t)(n % EX_STAGES) * (32 * 128), ga = g + c, ab = ga & 3;
-        const uint32_t ta = lane_base + 256 + 64 * ab;
+    for (int n = 0; ; ++n) {
+      request();  // into the patch read one chunk ago; the __syncwarp that closed that chunk orders the reads
+      if (n >= asked) break;
+      asm volatile("cp.async.wait_group %0;" :: "n"(EX_STAGES - 1) : "memory");
+      __syncwarp();
+      const uint32_t patch = patch0 + (uint32_t)(n % EX_STAGES) * (32 * 128), ga = 2 * n + par, ab = ga & 3;
+      const uint32_t ta = lane_base + 256 + 64 * ab;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x[16];
+      for (int h = 0; h < 4; ++h) {
+        float v[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 v = lds4(patch + lane * 128 + (((4 * h + i) ^ (lane & 7)) << 4));
-            x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
-          }
-          if (d.in_act) silu_fast_all(x, x);
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float t = to_tf32(x[i]);
-            hi[i] = __float_as_uint(t);
-            lo[i] = __float_as_uint(rest_tf32(x[i], t));
-          }
-          if (h == 0) {
-            if (ga >= 4 && alive) alive = mbar_wait(a_done + 8 * ab, ((ga >> 2) - 1) & 1);  // A buffer ab is free again
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          }
-          MB_TMEM_ST16(ta + 16 * h, hi);
-          MB_TMEM_ST16(ta + 32 + 16 * h, lo);
+        for (int i = 0; i < 2; ++i) {
+          const float4 f = lds4(patch + lane * 128 + (((2 * h + i) ^ (lane & 7)) << 4));
+          v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
         }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(a_ready + 8 * ab);
+        if (d.in_act) silu_fast_all(v, v);
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) split_tf32_even(v[i], hi[i], lo[i]);
+        if (h == 0) {
+          if (ga >= 4 && alive) alive = mbar_wait(a_done + 8 * ab, ((ga >> 2) - 1) & 1);  // A buffer ab is free again
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        MB_TMEM_ST8(ta + 8 * h, hi);
+        MB_TMEM_ST8(ta + 32 + 8 * h, lo);
       }
-      g += nch;
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(a_ready + 8 * ab);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
@@ -350,7 +344,7 @@ __global__ void __launch_bounds__(256) k_experts_split(int n_out, int n_in, int6
 #pragma unroll
   for (int i = ty; i < 32; i += 8) {
     const int64_t at = e0 + (int64_t)(n0 + i) * n_in + k0 + tx;
-    const float x = w[at], hi = to_tf32(x), lo = rest_tf32(x, hi);
+    const float x = w[at], hi = to_tf32(x), lo = to_tf32(x - hi);
     parts[at] = hi;
     parts[part + at] = lo;
     t[0][i][tx] = hi;
@@ -389,7 +383,7 @@ __global__ void __launch_bounds__(256) k_experts_split(int n_out, int n_in, int6
                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),        \
                  "=r"(v[15]) : "r"(taddr) : "memory")
 constexpr int EG_FLUSH = 4;
-constexpr int EG_AHEAD = 4;
+constexpr int EG_AHEAD = 10;
 constexpr int EG_BUFS = 4;
 constexpr int EG_BAR_OFF = EG_BUFS * 2 * TC_TILE_BYTES;
 constexpr int EG_SMEM_BYTES = EG_BAR_OFF + 256;
@@ -405,14 +399,17 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + EG_BAR_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + EG_BAR_OFF + 240);
+  // of an accumulator: -3 the run goes on, -2 / -1 it ends and is the share's first / second partial sum, e >= 0: all of expert e;
+  // -4: the share is done
+  volatile int32_t* const target = reinterpret_cast<volatile int32_t*>(smem + EG_BAR_OFF + 224);
   volatile uint32_t* const issued = reinterpret_cast<volatile uint32_t*>(smem + EG_BAR_OFF + 248);  // chunks whose products are under way
   if ((smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0) atomicOr(&g_gemm_status, 2);
     return;
   }
-  // ready[4] (8 column warps) done[4] | d_full[2] d_free[2] (8 epilogue warps) | retired
+  // ready[4] (8 column warps) done[4] | d_full[2] d_free[2] (8 epilogue warps) | retired | told[2] (where a finished accumulator goes)
   const uint32_t bar0 = smem_u32(bars);
-  const uint32_t ready = bar0, done = bar0 + 32, d_full = bar0 + 64, d_free = bar0 + 80, retired = bar0 + 96;
+  const uint32_t ready = bar0, done = bar0 + 32, d_full = bar0 + 64, d_free = bar0 + 80, retired = bar0 + 96, told = bar0 + 104;
   const uint32_t tiles = smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nk = d.n_in / 128, nb = nk * (d.n_out / 128);
@@ -422,7 +419,7 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
     if (lane == 0) {
       *issued = 0;
       for (int b = 0; b < 4; ++b) { mbar_init(ready + 8 * b, 8); mbar_init(done + 8 * b, 1); }
-      for (int b = 0; b < 2; ++b) { mbar_init(d_full + 8 * b, 1); mbar_init(d_free + 8 * b, 8); }
+      for (int b = 0; b < 2; ++b) { mbar_init(d_full + 8 * b, 1); mbar_init(d_free + 8 * b, 8); mbar_init(told + 8 * b, 1); }
       mbar_init(retired, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -450,13 +447,23 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0), tiles_u = __shfl_sync(0xffffffffu, tiles, 0);
     uint32_t g = 0, k = 0, in_acc = 0;
+    bool fresh = true, from_start = false;
+    auto tell = [&](int32_t what) {
+      if (lane == 0) {
+        target[k & 1] = what;
+        mbar_arrive(told + 8 * (k & 1));
+      }
+    };
     for (int64_t t = share.lo; t < share.hi && walk.seek((int)t, e, s0, left, first); ++t, ++g) {
       const uint32_t b = g & 3, acc = k & 1;
-      if (alive) alive = mbar_wait(ready + 8 * b, (g >> 2) & 1);
+      if (fresh) { from_start = first; fresh = false; }
       if (in_acc == 0 && k >= 2 && alive) alive = mbar_wait(d_free + 8 * acc, ((k >> 1) - 1) & 1);
+      if (alive) alive = mbar_wait(ready + 8 * b, (g >> 2) & 1);
       alive = __all_sync(0xffffffffu, alive);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const bool flush = in_acc == EG_FLUSH - 1 || left <= 32 || t + 1 == share.hi;
+      const bool end = left <= 32 || t + 1 == share.hi;
+      const bool flush = in_acc == EG_FLUSH - 1 || end;
+      if (flush) tell(!end ? -3 : from_start && left <= 32 ? e : from_start ? -1 : -2);
       if (elected) {
         issue_chunk_mmas<false>(tmem_u + 128u * acc, tmem_u + 256 + 64 * b, tiles_u + b * 2 * TC_TILE_BYTES, 0, in_acc == 0);
         mma_commit(done + 8 * b);
@@ -466,16 +473,27 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
       if (lane == 0) *issued = g + 1;
       ++in_acc;
       if (flush) { in_acc = 0; ++k; }
+      if (end) fresh = true;
     }
+    if (k >= 2 && alive) alive = mbar_wait(d_free + 8 * (k & 1), ((k >> 1) - 1) & 1);
+    tell(-4);
     drain_mma(retired, elected);
   } else if (warp == PS_TMA_WARP) {
     // lane = row of a chunk: four lines of dy, four of x.  A hint only: it waits for the products (a bounded number of naps) but nothing
-    // waits for it
-    for (int64_t t = share.lo; t < share.hi && walk.seek((int)t, e, s0, left, first); ++t) {
-      for (int naps = 0; naps < 1 << 16 && t - share.lo > (int64_t)*issued + EG_AHEAD; ++naps) __nanosleep(100);
-      if (lane < left) {
-        const float* const g = d.dy + (s0 + lane) * d.ld_dy + n0;
-        const float* const x = source_row(d, s0 + lane) + k0;
+    // waits for it.  The row numbers are read a chunk earlier still.
+    int32_t r = 0, r_next = 0;
+    int64_t s_next = 0, left_next = 0;
+    bool more = share.lo < share.hi;
+    for (int64_t t = share.lo; more || t == share.hi; ++t) {
+      const int64_t s = s_next, n = left_next;
+      r = r_next;
+      more = t < share.hi && walk.seek((int)t, e, s_next, left_next, first);
+      if (more && lane < left_next) r_next = d.idx ? d.idx[s_next + lane] : (int32_t)(s_next + lane);
+      if (t == share.lo) continue;
+      for (int naps = 0; naps < 1 << 17 && t - share.lo > (int64_t)*issued + EG_AHEAD; ++naps) __nanosleep(40);
+      if (lane < n) {
+        const float* const g = d.dy + (s + lane) * d.ld_dy + n0;
+        const float* const x = d.x + min(max((int64_t)r, (int64_t)0), d.n_rows - 1) * d.ld_x + k0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           asm volatile("prefetch.global.L2 [%0];" :: "l"(g + 32 * i));
@@ -491,17 +509,14 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
     f2 sum[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) sum[i] = two(0.f, 0.f);
-    uint32_t k = 0, in_acc = 0;
-    bool fresh = true, from_start = false;
-    for (int64_t t = share.lo; t < share.hi && walk.seek((int)t, e, s0, left, first); ++t) {
-      if (fresh) { from_start = first; fresh = false; }
-      const bool end = left <= 32 || t + 1 == share.hi;
-      if (++in_acc < EG_FLUSH && !end) continue;
-      in_acc = 0;
+    for (uint32_t k = 0; ; ++k) {
       const uint32_t acc = k & 1;
+      if (alive) alive = mbar_wait(told + 8 * acc, (k >> 1) & 1);
+      alive = __all_sync(0xffffffffu, alive);
+      const int what = alive ? target[acc] : -4;
+      if (what == -4) break;
       if (alive) alive = mbar_wait(d_full + 8 * acc, (k >> 1) & 1);
       alive = __all_sync(0xffffffffu, alive);
-      ++k;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
       for (int cg = 0; cg < 4; ++cg) {
@@ -514,17 +529,15 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(d_free + 8 * acc);
-      if (end) {
-        float* const out = (from_start && left <= 32 ? d.dw + e * whole : part + (2 * c + (from_start ? 1 : 0)) * whole) + at;
+      if (what == -3) continue;
+      float* const out = (what >= 0 ? d.dw + what * whole : part + (2 * c + 2 + what) * whole) + at;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float o[4];
-          apart(sum[2 * i], o[0], o[1]);
-          apart(sum[2 * i + 1], o[2], o[3]);
-          if (alive) st4(out + 4 * i, make_float4(o[0], o[1], o[2], o[3]));
-          sum[2 * i] = sum[2 * i + 1] = two(0.f, 0.f);
-        }
-        fresh = true;
+      for (int i = 0; i < 16; ++i) {
+        float o[4];
+        apart(sum[2 * i], o[0], o[1]);
+        apart(sum[2 * i + 1], o[2], o[3]);
+        if (alive) st4(out + 4 * i, make_float4(o[0], o[1], o[2], o[3]));
+        sum[2 * i] = sum[2 * i + 1] = two(0.f, 0.f);
       }
     }
   } else {
@@ -533,85 +546,87 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
     const int quarter = warp & 3, col = 32 * quarter + lane;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + 256;
     float v[32];               // this lane's column of a chunk; a half is asked for as soon as it has been used
-    Walk<5> ahead = walk;
-    int64_t t_ask = share.lo, next_ld = is_x ? d.ld_x : d.ld_dy;
-    int rows = 0, row = 0;     // of the chunk asked for; x: lane's source row
+    // chunk 1: asked for, with its rows' number, row of this lane, address of this lane's column; chunk 2: the one after it
+    int rows1 = 0, rows2 = 0, row1 = 0, row2 = 0;
+    int64_t t_next = share.lo, s2 = 0;
     const float* next = nullptr;
-    auto look_up = [&]() {
-      int e_;
-      int64_t s_;
-      rows = 0;
-      if (t_ask >= share.hi || !ahead.seek((int)t_ask++, e_, s_, rows)) return;
-      if (is_x) {
-        row = lane < rows ? (d.idx ? d.idx[s_ + lane] : (int32_t)(s_ + lane)) : 0;
-        row = (int32_t)min(max((int64_t)row, (int64_t)0), d.n_rows - 1);
-        next = d.x + k0 + col;
-      } else {
-        row = lane;
-        next = d.dy + s_ * d.ld_dy + n0 + col;
+    const int ld = (int)(is_x ? d.ld_x : d.ld_dy);
+    const float* const base = is_x ? d.x + k0 + col : d.dy + n0 + col;
+    int e1 = 0, e2 = 0;        // what the bias gradient needs: expert, whether the chunk is its first / its last
+    bool first1 = false, first2 = false, last1 = false, last2 = false;
+    auto look_up = [&]() {     // chunk 2 becomes chunk 1, and a new one is looked up
+      rows1 = rows2; e1 = e2; first1 = first2; last1 = last2;
+      row1 = (int)min(max((int64_t)row2, (int64_t)0), d.n_rows - 1);
+      next = is_x ? base : base + s2 * d.ld_dy;
+      rows2 = 0;
+      int64_t left_;
+      if (t_next < share.hi && walk.seek((int)t_next, e2, s2, left_, first2)) {
+        last2 = left_ <= 32;
+        rows2 = last2 ? (int)left_ : 32;
+        if (is_x && lane < rows2) row2 = d.idx ? d.idx[s2 + lane] : (int32_t)(s2 + lane);
       }
+      ++t_next;
     };
     auto ask = [&](int h) {
+      if (rows1 == 32) {
 #pragma unroll
-      for (int i = 16 * h; i < 16 * h + 16; ++i) {
-        const int64_t r = is_x ? __shfl_sync(0xffffffffu, row, i) : i;
-        v[i] = i < rows ? next[r * next_ld] : 0.f;
+        for (int i = 8 * h; i < 8 * h + 8; ++i) v[i] = next[(int64_t)(is_x ? __shfl_sync(0xffffffffu, row1, i) : i) * ld];
+      } else {
+#pragma unroll
+        for (int i = 8 * h; i < 8 * h + 8; ++i) {
+          const int r = is_x ? __shfl_sync(0xffffffffu, row1, i) : i;
+          v[i] = i < rows1 ? next[(int64_t)r * ld] : 0.f;
+        }
       }
     };
     look_up();
-    ask(0);
-    ask(1);
+    look_up();
+#pragma unroll
+    for (int h = 0; h < 4; ++h) ask(h);
     uint32_t g = 0;
     float bias = 0.f;
     bool fresh = true, from_start = false;
-    for (int64_t t = share.lo; t < share.hi && walk.seek((int)t, e, s0, left, first); ++t, ++g) {
+    for (int64_t t = share.lo; t < share.hi; ++t, ++g) {
       const uint32_t b = g & 3;
+      const int e0 = e1;
+      const bool first0 = first1, last0 = last1;
       look_up();
       if (g >= 4 && alive) alive = mbar_wait(done + 8 * b, ((g >> 2) - 1) & 1);
       alive = __all_sync(0xffffffffu, alive);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t line = tiles + b * 2 * TC_TILE_BYTES + col * 128;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t hi[16], lo[16];
-        float x[16];
+      for (int h = 0; h < 4; ++h) {
+        uint32_t hi[8], lo[8];
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = v[16 * h + i];
+        for (int i = 0; i < 8; ++i) x[i] = v[8 * h + i];
         if (is_x && d.in_act) silu_fast_all(x, x);
-        if (!is_x) {
-          float sum = 0.f;
+        if (!is_x) bias += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) sum += (x[i] + x[i + 1]) + (x[i + 2] + x[i + 3]);
-          bias += sum;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float f = to_tf32(x[i]);
-          hi[i] = __float_as_uint(f);
-          lo[i] = __float_as_uint(rest_tf32(x[i], f));
-        }
+        for (int i = 0; i < 8; ++i) split_tf32_even(x[i], hi[i], lo[i]);
         if (is_x) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t to = line + (((4 * h + i) ^ (col & 7)) << 4);
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t to = line + (((2 * h + i) ^ (col & 7)) << 4);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
                          :: "r"(to), "r"(hi[4 * i]), "r"(hi[4 * i + 1]), "r"(hi[4 * i + 2]), "r"(hi[4 * i + 3]) : "memory");
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
                          :: "r"(to + TC_TILE_BYTES), "r"(lo[4 * i]), "r"(lo[4 * i + 1]), "r"(lo[4 * i + 2]), "r"(lo[4 * i + 3]) : "memory");
           }
         } else {
-          MB_TMEM_ST16(lane_base + 64 * b + 16 * h, hi);
-          MB_TMEM_ST16(lane_base + 64 * b + 32 + 16 * h, lo);
+          MB_TMEM_ST8(lane_base + 64 * b + 8 * h, hi);
+          MB_TMEM_ST8(lane_base + 64 * b + 32 + 8 * h, lo);
         }
         ask(h);
       }
       if (is_x) {
         to_async_proxy();
       } else {
-        if (fresh) { from_start = first; fresh = false; }
-        if (left <= 32 || t + 1 == share.hi) {
+        if (fresh) { from_start = first0; fresh = false; }
+        if (last0 || t + 1 == share.hi) {
           if (part_bias && k0 == 0) {
-            float* const out = from_start && left <= 32 ? d.dbias + (int64_t)e * d.n_out : part_bias + (int64_t)(2 * c + (from_start ? 1 : 0)) * d.n_out;
+            float* const out = from_start && last0 ? d.dbias + (int64_t)e0 * d.n_out : part_bias + (int64_t)(2 * c + (from_start ? 1 : 0)) * d.n_out;
             out[n0 + col] = bias;
           }
           bias = 0.f;

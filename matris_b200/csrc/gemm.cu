@@ -1441,7 +1441,7 @@ extern "C" int mb_mlp_bwd_data(const mb_mlp_bwd* g, void* stream_) {
 // ------------------------------------------------------------------ experts
 namespace mb {
 static bool aligned_rows(const void* p, int64_t ld, int width) {
-  return p && (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 4 == 0 && ld >= width;
+  return p && (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 4 == 0 && ld >= width && ld <= INT32_MAX;
 }
 static bool experts_valid(const mb_experts* d) {
   return d && d->n_slots >= 0 && d->n_slots <= INT32_MAX && d->n_rows >= 0 && d->n_experts >= 1 && d->n_experts <= EX_MAX_EXPERTS &&
