@@ -72,6 +72,16 @@ template <int SHIFT> struct Walk {
     rows = left < (1 << SHIFT) ? (int)left : 1 << SHIFT;
     return true;
   }
+  // the tile after the one that (e, s0, left) describes, number t: without a search while the expert lasts
+  __device__ __forceinline__ bool next(int t, int& e, int64_t& s0, int64_t& left, bool& first) {
+    if (left > (1 << SHIFT)) {
+      s0 += 1 << SHIFT;
+      left -= 1 << SHIFT;
+      first = false;
+      return true;
+    }
+    return seek(t, e, s0, left, first);
+  }
   // all tiles; the walk is at the start again
   __device__ __forceinline__ int64_t count() {
     int64_t n = 0;
@@ -374,8 +384,7 @@ __global__ void __launch_bounds__(256) k_experts_split(int n_out, int n_in, int6
 // short by up to n 2^-23.  So a run is accumulated there for EG_FLUSH chunks only and added up in float32 registers of the epilogue
 // warps, rounded to nearest.
 //
-// Roles: warp 0 issues the products, warp 1 asks L2 for the rows four chunks ahead, warps 2 - 5 hold dy's columns, 6 - 9 x's, 10 - 17
-// the sums.
+// Roles: warp 0 issues the products, warps 2 - 5 hold dy's columns, 6 - 9 x's, 10 - 17 the sums (warp 1 has none).
 #define MB_TMEM_LD16(taddr, v)                                                                                   \
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "                                                         \
                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"                  \
@@ -383,10 +392,12 @@ __global__ void __launch_bounds__(256) k_experts_split(int n_out, int n_in, int6
                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),        \
                  "=r"(v[15]) : "r"(taddr) : "memory")
 constexpr int EG_FLUSH = 4;
-constexpr int EG_AHEAD = 10;
 constexpr int EG_BUFS = 4;
-constexpr int EG_BAR_OFF = EG_BUFS * 2 * TC_TILE_BYTES;
+constexpr int EG_STAGES = 3;
+constexpr int EG_PATCH_OFF = EG_BUFS * 2 * TC_TILE_BYTES;
+constexpr int EG_BAR_OFF = EG_PATCH_OFF + 8 * EG_STAGES * 32 * 128;
 constexpr int EG_SMEM_BYTES = EG_BAR_OFF + 256;
+static_assert(EG_SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
 
 struct GradShare {  // chunks [lo, hi) of share c of n
   int64_t all, lo, hi;
@@ -402,7 +413,6 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
   // of an accumulator: -3 the run goes on, -2 / -1 it ends and is the share's first / second partial sum, e >= 0: all of expert e;
   // -4: the share is done
   volatile int32_t* const target = reinterpret_cast<volatile int32_t*>(smem + EG_BAR_OFF + 224);
-  volatile uint32_t* const issued = reinterpret_cast<volatile uint32_t*>(smem + EG_BAR_OFF + 248);  // chunks whose products are under way
   if ((smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0) atomicOr(&g_gemm_status, 2);
     return;
@@ -417,7 +427,6 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
 
   if (warp == PS_MMA_WARP) {
     if (lane == 0) {
-      *issued = 0;
       for (int b = 0; b < 4; ++b) { mbar_init(ready + 8 * b, 8); mbar_init(done + 8 * b, 1); }
       for (int b = 0; b < 2; ++b) { mbar_init(d_full + 8 * b, 1); mbar_init(d_free + 8 * b, 8); mbar_init(told + 8 * b, 1); }
       mbar_init(retired, 1);
@@ -454,7 +463,8 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
         mbar_arrive(told + 8 * (k & 1));
       }
     };
-    for (int64_t t = share.lo; t < share.hi && walk.seek((int)t, e, s0, left, first); ++t, ++g) {
+    left = 0;
+    for (int64_t t = share.lo; t < share.hi && walk.next((int)t, e, s0, left, first); ++t, ++g) {
       const uint32_t b = g & 3, acc = k & 1;
       if (fresh) { from_start = first; fresh = false; }
       if (in_acc == 0 && k >= 2 && alive) alive = mbar_wait(d_free + 8 * acc, ((k >> 1) - 1) & 1);
@@ -470,7 +480,6 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
         if (flush) mma_commit(d_full + 8 * acc);
       }
       __syncwarp();
-      if (lane == 0) *issued = g + 1;
       ++in_acc;
       if (flush) { in_acc = 0; ++k; }
       if (end) fresh = true;
@@ -478,29 +487,6 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
     if (k >= 2 && alive) alive = mbar_wait(d_free + 8 * (k & 1), ((k >> 1) - 1) & 1);
     tell(-4);
     drain_mma(retired, elected);
-  } else if (warp == PS_TMA_WARP) {
-    // lane = row of a chunk: four lines of dy, four of x.  A hint only: it waits for the products (a bounded number of naps) but nothing
-    // waits for it.  The row numbers are read a chunk earlier still.
-    int32_t r = 0, r_next = 0;
-    int64_t s_next = 0, left_next = 0;
-    bool more = share.lo < share.hi;
-    for (int64_t t = share.lo; more || t == share.hi; ++t) {
-      const int64_t s = s_next, n = left_next;
-      r = r_next;
-      more = t < share.hi && walk.seek((int)t, e, s_next, left_next, first);
-      if (more && lane < left_next) r_next = d.idx ? d.idx[s_next + lane] : (int32_t)(s_next + lane);
-      if (t == share.lo) continue;
-      for (int naps = 0; naps < 1 << 17 && t - share.lo > (int64_t)*issued + EG_AHEAD; ++naps) __nanosleep(40);
-      if (lane < n) {
-        const float* const g = d.dy + (s + lane) * d.ld_dy + n0;
-        const float* const x = d.x + min(max((int64_t)r, (int64_t)0), d.n_rows - 1) * d.ld_x + k0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          asm volatile("prefetch.global.L2 [%0];" :: "l"(g + 32 * i));
-          asm volatile("prefetch.global.L2 [%0];" :: "l"(x + 32 * i));
-        }
-      }
-    }
   } else if (warp >= PS_EPI_WARP0) {
     // thread = row of the block, 64 of its columns; sums of a run in registers
     const int quarter = warp & 3, half = (warp - PS_EPI_WARP0) >> 2;
@@ -540,57 +526,62 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
         sum[2 * i] = sum[2 * i + 1] = two(0.f, 0.f);
       }
     }
-  } else {
+  } else if (warp >= PS_PROD_WARP0) {
     // columns: warps 2 - 5 dy (A, tensor memory), 6 - 9 x (B, shared memory), 32 columns each
     const bool is_x = warp >= PS_PROD_WARP0 + 4;
     const int quarter = warp & 3, col = 32 * quarter + lane;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + 256;
-    float v[32];               // this lane's column of a chunk; a half is asked for as soon as it has been used
-    // chunk 1: asked for, with its rows' number, row of this lane, address of this lane's column; chunk 2: the one after it
-    int rows1 = 0, rows2 = 0, row1 = 0, row2 = 0;
-    int64_t t_next = share.lo, s2 = 0;
-    const float* next = nullptr;
+    // A chunk's 32 rows x 32 columns come by cp.async into a patch of the warp's own, EG_STAGES - 1 chunks ahead, and are read back by
+    // column: 32 lanes, 32 neighbouring words.  (With plain loads into registers a chunk ahead the warps waited for the loads just
+    // issued: 717 us where this takes 300.)
+    const int lr = lane >> 3, lc = lane & 7;
+    const uint32_t patch0 = tiles + EG_PATCH_OFF + (warp - PS_PROD_WARP0) * (EG_STAGES * 32 * 128);
+    int row = 0, asked = 0;    // lane's row of the next chunk to ask for (x: in the source), looked up a chunk earlier
+    int rows = 0;
+    int64_t t_next = share.lo;
+    const float* const base = (is_x ? d.x + k0 : d.dy + n0) + 32 * quarter + 4 * lc;
     const int ld = (int)(is_x ? d.ld_x : d.ld_dy);
-    const float* const base = is_x ? d.x + k0 + col : d.dy + n0 + col;
-    int e1 = 0, e2 = 0;        // what the bias gradient needs: expert, whether the chunk is its first / its last
-    bool first1 = false, first2 = false, last1 = false, last2 = false;
-    auto look_up = [&]() {     // chunk 2 becomes chunk 1, and a new one is looked up
-      rows1 = rows2; e1 = e2; first1 = first2; last1 = last2;
-      row1 = (int)min(max((int64_t)row2, (int64_t)0), d.n_rows - 1);
-      next = is_x ? base : base + s2 * d.ld_dy;
-      rows2 = 0;
-      int64_t left_;
-      if (t_next < share.hi && walk.seek((int)t_next, e2, s2, left_, first2)) {
-        last2 = left_ <= 32;
-        rows2 = last2 ? (int)left_ : 32;
-        if (is_x && lane < rows2) row2 = d.idx ? d.idx[s2 + lane] : (int32_t)(s2 + lane);
+    left = 0;
+    auto look_up = [&]() {
+      rows = 0;
+      if (t_next < share.hi && walk.next((int)t_next, e, s0, left, first)) {
+        rows = left < 32 ? (int)left : 32;
+        row = lane < rows ? (is_x && d.idx ? d.idx[s0 + lane] : (int32_t)(s0 + lane)) : 0;
       }
       ++t_next;
     };
-    auto ask = [&](int h) {
-      if (rows1 == 32) {
+    auto request = [&]() {
+      if (rows > 0) {
+        const int r = is_x ? (int)min(max((int64_t)row, (int64_t)0), d.n_rows - 1) : row;
+        const uint32_t to = patch0 + (uint32_t)(asked % EG_STAGES) * (32 * 128) + lr * 128 + lc * 16;
 #pragma unroll
-        for (int i = 8 * h; i < 8 * h + 8; ++i) v[i] = next[(int64_t)(is_x ? __shfl_sync(0xffffffffu, row1, i) : i) * ld];
-      } else {
-#pragma unroll
-        for (int i = 8 * h; i < 8 * h + 8; ++i) {
-          const int r = is_x ? __shfl_sync(0xffffffffu, row1, i) : i;
-          v[i] = i < rows1 ? next[(int64_t)r * ld] : 0.f;
+        for (int i = 0; i < 8; ++i) {
+          const float* const from = base + (int64_t)__shfl_sync(0xffffffffu, r, lr + 4 * i) * ld;
+          const int bytes = lr + 4 * i < rows ? 16 : 0;  // 0: nothing is read, zeros are written
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to + 512u * i), "l"(from), "r"(bytes) : "memory");
         }
+        ++asked;
+        look_up();
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
     look_up();
-    look_up();
-#pragma unroll
-    for (int h = 0; h < 4; ++h) ask(h);
+    for (int i = 0; i < EG_STAGES - 1; ++i) request();
+    // what the bias gradient needs, chunk by chunk, from a walk of its own
+    Walk<5> now = walk;
+    int e0 = 0;
+    int64_t now_s = 0, now_left = 0;
+    bool first0 = false;
+    if (!is_x) { now.start(d); }
     uint32_t g = 0;
     float bias = 0.f;
     bool fresh = true, from_start = false;
     for (int64_t t = share.lo; t < share.hi; ++t, ++g) {
       const uint32_t b = g & 3;
-      const int e0 = e1;
-      const bool first0 = first1, last0 = last1;
-      look_up();
+      request();  // into the patch read one chunk ago; the __syncwarp that closed that chunk orders the reads
+      asm volatile("cp.async.wait_group %0;" :: "n"(EG_STAGES - 1) : "memory");
+      __syncwarp();
+      const uint32_t patch = patch0 + (g % EG_STAGES) * (32 * 128) + lane * 4;
       if (g >= 4 && alive) alive = mbar_wait(done + 8 * b, ((g >> 2) - 1) & 1);
       alive = __all_sync(0xffffffffu, alive);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -600,7 +591,7 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
         uint32_t hi[8], lo[8];
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = v[8 * h + i];
+        for (int i = 0; i < 8; ++i) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x[i]) : "r"(patch + 128u * (8 * h + i)) : "memory");
         if (is_x && d.in_act) silu_fast_all(x, x);
         if (!is_x) bias += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
@@ -618,11 +609,12 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
           MB_TMEM_ST8(lane_base + 64 * b + 8 * h, hi);
           MB_TMEM_ST8(lane_base + 64 * b + 32 + 8 * h, lo);
         }
-        ask(h);
       }
       if (is_x) {
         to_async_proxy();
       } else {
+        now.next((int)t, e0, now_s, now_left, first0);
+        const bool last0 = now_left <= 32;
         if (fresh) { from_start = first0; fresh = false; }
         if (last0 || t + 1 == share.hi) {
           if (part_bias && k0 == 0) {
