@@ -27,7 +27,32 @@ __device__ __forceinline__ const float* source_row(const mb_experts& d, int64_t 
 //
 // shared (K = 128): the four A buffers hold the whole row tile, converted once for all its column blocks.  Otherwise a column block is a
 // tile of its own and its rows are gathered again, from L2.
+#define MB_TMEM_LD16(taddr, v)                                                                                   \
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "                                                         \
+               "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"                  \
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), \
+                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),        \
+                 "=r"(v[15]) : "r"(taddr) : "memory")
 struct alignas(64) ExMaps { CUtensorMap hi, lo; };
+
+// Whether a phase is over, without waiting for it
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+// The products of K steps [from, to) of a chunk (four of them): A in tensor memory at ta (hi | lo), weight or column tiles at wb (hi | lo)
+__device__ __forceinline__ void chunk_products(uint32_t d_tmem, uint32_t ta, uint32_t wb, int from, int to, bool fresh) {
+  const uint64_t dbh = umma_desc(wb), dbl = umma_desc(wb + TC_TILE_BYTES);
+#pragma unroll
+  for (int kk = from; kk < to; ++kk) {
+    const uint64_t adv = (uint64_t)(2 * kk);
+    umma_tf32_ts(d_tmem, ta + 32 + 8 * kk, dbh + adv, (!fresh || kk > 0) ? 1u : 0u);
+    umma_tf32_ts(d_tmem, ta + 8 * kk, dbl + adv, 1u);
+    umma_tf32_ts(d_tmem, ta + 8 * kk, dbh + adv, 1u);
+  }
+}
 
 // Tiles of 2^SHIFT slots in order of expert; all lanes of a warp call it together
 template <int SHIFT> struct Walk {
@@ -92,9 +117,13 @@ template <int SHIFT> struct Walk {
   }
 };
 
-constexpr int EX_STAGES = 3;                                     // patches of a producer warp
-constexpr int EX_PATCH_BYTES = 8 * EX_STAGES * 32 * 128;
-constexpr int EX_BAR_OFF = PS_RING_BYTES + EX_PATCH_BYTES;
+// A producer warp spends some 2,500 cycles on a chunk of 32 x 32 values, most of them waiting for its own instructions, where the chunk's
+// products take 768: sixteen of them, each chunk of four to a set of its own (eight, of two: 200 us where this takes 150).
+constexpr int EX_SETS = 4, EX_PROD_WARPS = 4 * EX_SETS, EX_EPI_WARP0 = PS_PROD_WARP0 + EX_PROD_WARPS, EX_THREADS = 32 * (EX_EPI_WARP0 + 8);
+constexpr int EX_STAGES = 2;                                     // patches of a producer warp
+constexpr int EX_W_SLOTS = 3;                                    // weight tiles (hi and lo) in flight
+constexpr int EX_PATCH_OFF = EX_W_SLOTS * 2 * TC_TILE_BYTES;
+constexpr int EX_BAR_OFF = EX_PATCH_OFF + EX_PROD_WARPS * EX_STAGES * 32 * 128;
 constexpr int EX_SMEM_BYTES = EX_BAR_OFF + 256;
 static_assert(EX_SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
 
@@ -105,7 +134,7 @@ __device__ __forceinline__ void split_tf32_even(float x, uint32_t& hi, uint32_t&
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
-__global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant__ mb_experts d, const __grid_constant__ ExMaps maps, const int shared) {
+__global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant__ mb_experts d, const __grid_constant__ ExMaps maps, const int shared) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + EX_BAR_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + EX_BAR_OFF + 240);
@@ -113,7 +142,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
     if (threadIdx.x == 0) atomicOr(&g_gemm_status, 2);
     return;
   }
-  // a_ready[4] (4 producer warps) a_done[4] | w_ready[4] w_done[4] | d_full[2] d_free[2] (8 epilogue warps) | retired
+  // a_ready[4] (4 producer warps) a_done[4] | w_ready[3] w_done[3] | d_full[2] d_free[2] (8 epilogue warps) | retired
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t a_ready = bar0, a_done = bar0 + 32, w_ready = bar0 + 64, w_done = bar0 + 96, d_full = bar0 + 128, d_free = bar0 + 144,
                  retired = bar0 + 160;
@@ -126,7 +155,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
   if (warp == PS_MMA_WARP) {
     if (lane == 0) {
       for (int b = 0; b < 4; ++b) { mbar_init(a_ready + 8 * b, 4); mbar_init(a_done + 8 * b, 1); }
-      for (int b = 0; b < 4; ++b) { mbar_init(w_ready + 8 * b, 1); mbar_init(w_done + 8 * b, 1); }
+      for (int b = 0; b < EX_W_SLOTS; ++b) { mbar_init(w_ready + 8 * b, 1); mbar_init(w_done + 8 * b, 1); }
       for (int b = 0; b < 2; ++b) { mbar_init(d_full + 8 * b, 1); mbar_init(d_free + 8 * b, 8); }
       mbar_init(retired, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -151,25 +180,48 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
     uint32_t elected;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0), ring_u = __shfl_sync(0xffffffffu, ring, 0);
+    // The number of this CTA's items, from one lane: the loop, and with it every operand of a matrix instruction, is then the same for all
+    // lanes by construction.  Where the compiler cannot see that it moves each operand to a uniform register in front of each instruction
+    // (walking the tiles here took 1,440 cycles a chunk for 768 of products).
+    const int64_t items = walk.count() * per_tile;
+    const int n_items = __shfl_sync(0xffffffffu, (int)((items - blockIdx.x + gridDim.x - 1) / gridDim.x), 0);
     bool alive = true;
-    uint32_t g = 0, wu = 0, k = 0;  // A chunks, weight slots, column blocks so far
-    for (int item = blockIdx.x; walk.seek(item / per_tile, e, s0, rows); item += gridDim.x) {
+    uint32_t g = 0, k = 0, slot = 0, phase = 0;  // A chunks and column blocks so far; weight slot and its use
+    // The tensor cores' queue is a few instructions deep: issuing a chunk's twelve takes as long as they do, and then a wait that finds its
+    // barrier open still takes 110 - 140 cycles, three of them a chunk.  So the next chunk's barriers are tested ahead of the last
+    // three instructions, and waited for only where that fails (200 -> 165 us).
+    bool open = false;
+    for (int it = 0; it < n_items; ++it) {
       for (int j = 0; j < per_item; ++j, ++k) {
         const uint32_t acc = k & 1, d_tmem = tmem_u + 128u * acc;
-        for (int c = 0; c < nch; ++c, ++wu) {
-          const uint32_t ga = g + c, ab = ga & 3, slot = wu & 3;
-          if (j == 0 && alive) alive = mbar_wait(a_ready + 8 * ab, (ga >> 2) & 1);
-          if (alive) alive = mbar_wait(w_ready + 8 * slot, (wu >> 2) & 1);
-          if (c == 0 && k >= 2 && alive) alive = mbar_wait(d_free + 8 * acc, ((k >> 1) - 1) & 1);
-          alive = __all_sync(0xffffffffu, alive);
+        for (int c = 0; c < nch; ++c) {
+          const uint32_t ga = g + c, ab = ga & 3;
+          if (!open) {
+            if (j == 0 && alive) alive = mbar_wait(a_ready + 8 * ab, (ga >> 2) & 1);
+            if (alive) alive = mbar_wait(w_ready + 8 * slot, phase & 1);
+            if (c == 0 && k >= 2 && alive) alive = mbar_wait(d_free + 8 * acc, ((k >> 1) - 1) & 1);
+            alive = __all_sync(0xffffffffu, alive);
+          }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t ta = tmem_u + 256 + 64 * ab, wb = ring_u + slot * 2 * TC_TILE_BYTES;
+          if (elected) chunk_products(d_tmem, ta, wb, 0, 3, c == 0);
+          __syncwarp();
+          const uint32_t slot1 = slot + 1 == EX_W_SLOTS ? 0 : slot + 1, phase1 = slot1 == 0 ? phase + 1 : phase;
+          const bool block_ends = c == nch - 1, item_ends = block_ends && j == per_item - 1;
+          const uint32_t k1 = k + 1, g1 = ga + 1;
+          bool ok = mbar_test(w_ready + 8 * slot1, phase1 & 1);
+          if (item_ends || (!block_ends && j == 0)) ok = mbar_test(a_ready + 8 * (g1 & 3), (g1 >> 2) & 1) && ok;
+          if (block_ends && k1 >= 2) ok = mbar_test(d_free + 8 * (k1 & 1), ((k1 >> 1) - 1) & 1) && ok;
+          open = __all_sync(0xffffffffu, ok);
           if (elected) {
-            issue_chunk_mmas<false>(d_tmem, tmem_u + 256 + 64 * ab, ring_u + slot * 2 * TC_TILE_BYTES, 0, c == 0);
+            chunk_products(d_tmem, ta, wb, 3, 4, false);
             if (j == per_item - 1) mma_commit(a_done + 8 * ab);
             mma_commit(w_done + 8 * slot);
-            if (c == nch - 1) mma_commit(d_full + 8 * acc);
+            if (block_ends) mma_commit(d_full + 8 * acc);
           }
           __syncwarp();
+          slot = slot1;
+          phase = phase1;
         }
       }
       g += nch;
@@ -180,13 +232,12 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
     const uint32_t ring_u = __shfl_sync(0xffffffffu, ring, 0);
     bool alive = true;
-    uint32_t wu = 0;
+    uint32_t wu = 0, slot = 0, phase = 0;
     for (int item = blockIdx.x; alive && walk.seek(item / per_tile, e, s0, rows); item += gridDim.x) {
       for (int j = 0; j < per_item && alive; ++j) {
         const int row = e * d.n_out + 128 * (shared ? j : item % nb);
         for (int c = 0; c < nch; ++c, ++wu) {
-          const uint32_t slot = wu & 3;
-          if (wu >= 4) alive = mbar_wait(w_done + 8 * slot, ((wu >> 2) - 1) & 1);
+          if (phase > 0) alive = mbar_wait(w_done + 8 * slot, (phase - 1) & 1);
           alive = __all_sync(0xffffffffu, alive);
           if (!alive) break;
           if (elected) {
@@ -196,13 +247,14 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
             tma_load_2d(dst + TC_TILE_BYTES, &maps.lo, bar, c * TC_BK, row);
           }
           __syncwarp();
+          if (++slot == EX_W_SLOTS) { slot = 0; ++phase; }
         }
       }
     }
-    drain_copies(w_ready, 4, wu);
-  } else if (warp >= PS_EPI_WARP0) {
+    drain_copies(w_ready, EX_W_SLOTS, wu);
+  } else if (warp >= EX_EPI_WARP0) {
     // thread = row; epilogue warp e takes columns 64 (e >> 2).. of the accumulator
-    const int quarter = warp & 3, half = (warp - PS_EPI_WARP0) >> 2;
+    const int quarter = warp & 3, half = (warp - EX_EPI_WARP0) >> 2;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 64);
     const bool wide = ((reinterpret_cast<uintptr_t>(d.y) | reinterpret_cast<uintptr_t>(d.gate)) & 31u) == 0 && d.ld_y % 8 == 0 && d.ld_gate % 8 == 0;
     bool alive = true;
@@ -224,19 +276,19 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
         alive = __all_sync(0xffffffffu, alive);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-        for (int cg = 0; cg < 2; ++cg) {
-          uint32_t v[32];
-          MB_TMEM_LD32(lane_base + 128u * acc + 32u * cg, v);
+        for (int cg = 0; cg < 4; ++cg) {
+          uint32_t v[16];
+          MB_TMEM_LD16(lane_base + 128u * acc + 16u * cg, v);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          if (cg == 1) {
+          if (cg == 3) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(d_free + 8 * acc);
           }
           if (!alive || !valid) continue;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int c = cg * 32 + q * 8;
+          for (int q = 0; q < 2; ++q) {
+            const int c = cg * 16 + q * 8;
             float o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(v[8 * q + i]);
@@ -258,17 +310,18 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
       }
     }
   } else {
-    // producers: lane quarter, K chunks of this warp's parity; thread = row = TMEM lane
-    const int pw = warp - PS_PROD_WARP0, par = pw >> 2, quarter = warp & 3, lr = lane >> 3, lc = lane & 7;
+    // producers: lane quarter, every fourth K chunk; thread = row = TMEM lane
+    const int pw = warp - PS_PROD_WARP0, set = pw >> 2, quarter = warp & 3, lr = lane >> 3, lc = lane & 7;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t patch0 = smem_u32(smem + PS_RING_BYTES + pw * (EX_STAGES * 32 * 128));
+    const uint32_t patch0 = smem_u32(smem + EX_PATCH_OFF + pw * (EX_STAGES * 32 * 128));
     const uint32_t put_even = lr * 128 + ((lc ^ lr) << 4), put_odd = lr * 128 + ((lc ^ (lr | 4)) << 4);
     // The walk is that of the chunks asked for, EX_STAGES - 1 ahead of those converted; the rows of an item are looked up a chunk before
-    // they are needed.  This warp's n-th chunk is chunk 2 n + par of the CTA.
+    // they are needed.  This warp's n-th chunk is chunk 4 n + set of the CTA
+    // and goes to A buffer `set`.
     int item = blockIdx.x, g_c = 0, asked = 0;
     int32_t a_row[8], next_row[8];
     bool more;
-    const float* const x = d.x + par * TC_BK + 4 * lc;
+    const float* const x = d.x + set * TC_BK + 4 * lc;
     auto look_up = [&]() {
       more = walk.seek(item / per_tile, e, s0, rows);
       if (!more) return;
@@ -286,11 +339,11 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
           for (int i = 0; i < 8; ++i) a_row[i] = (int32_t)min(max((int64_t)next_row[i], (int64_t)0), d.n_rows - 1);
         }
         const uint32_t to = patch0 + (uint32_t)(asked % EX_STAGES) * (32 * 128);
-        const float* const from = x + 2 * TC_BK * g_c;
+        const float* const from = x + EX_SETS * TC_BK * g_c;
 #pragma unroll
         for (int i = 0; i < 8; ++i) copy16(to + ((i & 1) ? put_odd : put_even) + 512u * i, from + (int64_t)a_row[i] * (int)d.ld_x);
         ++asked;
-        if (++g_c == nch / 2) { g_c = 0; item += gridDim.x; look_up(); }
+        if (++g_c == nch / EX_SETS) { g_c = 0; item += gridDim.x; look_up(); }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -302,8 +355,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
       if (n >= asked) break;
       asm volatile("cp.async.wait_group %0;" :: "n"(EX_STAGES - 1) : "memory");
       __syncwarp();
-      const uint32_t patch = patch0 + (uint32_t)(n % EX_STAGES) * (32 * 128), ga = 2 * n + par, ab = ga & 3;
-      const uint32_t ta = lane_base + 256 + 64 * ab;
+      const uint32_t patch = patch0 + (uint32_t)(n % EX_STAGES) * (32 * 128), ta = lane_base + 256 + 64 * set;
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         float v[8];
@@ -317,7 +369,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
 #pragma unroll
         for (int i = 0; i < 8; ++i) split_tf32_even(v[i], hi[i], lo[i]);
         if (h == 0) {
-          if (ga >= 4 && alive) alive = mbar_wait(a_done + 8 * ab, ((ga >> 2) - 1) & 1);  // A buffer ab is free again
+          if (n > 0 && alive) alive = mbar_wait(a_done + 8 * set, (n - 1) & 1);  // the A buffer is free again
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
         MB_TMEM_ST8(ta + 8 * h, hi);
@@ -326,14 +378,14 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_experts(const __grid_constant
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(a_ready + 8 * ab);
+      if (lane == 0) mbar_arrive(a_ready + 8 * set);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
 
   if (d.zero_rest) {  // slots behind the last
     const int64_t used = min(max((int64_t)d.offsets[d.n_experts], (int64_t)0), d.n_slots);
-    for (int64_t s = used + (int64_t)blockIdx.x * (PS_THREADS / 32) + warp; s < d.n_slots; s += (int64_t)gridDim.x * (PS_THREADS / 32))
+    for (int64_t s = used + (int64_t)blockIdx.x * (EX_THREADS / 32) + warp; s < d.n_slots; s += (int64_t)gridDim.x * (EX_THREADS / 32))
       for (int c = 4 * lane; c < d.n_out; c += 128) st4(d.y + s * d.ld_y + c, make_float4(0.f, 0.f, 0.f, 0.f));
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -385,12 +437,6 @@ __global__ void __launch_bounds__(256) k_experts_split(int n_out, int n_in, int6
 // warps, rounded to nearest.
 //
 // Roles: warp 0 issues the products, warps 2 - 5 hold dy's columns, 6 - 9 x's, 10 - 17 the sums (warp 1 has none).
-#define MB_TMEM_LD16(taddr, v)                                                                                   \
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "                                                         \
-               "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"                  \
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), \
-                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),        \
-                 "=r"(v[15]) : "r"(taddr) : "memory")
 constexpr int EG_FLUSH = 4;
 constexpr int EG_BUFS = 4;
 constexpr int EG_STAGES = 3;
@@ -474,10 +520,13 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
       const bool end = left <= 32 || t + 1 == share.hi;
       const bool flush = in_acc == EG_FLUSH - 1 || end;
       if (flush) tell(!end ? -3 : from_start && left <= 32 ? e : from_start ? -1 : -2);
+      // from one lane, so that the operands of the matrix instructions are the same for all by construction (see k_experts)
+      const uint32_t how = __shfl_sync(0xffffffffu, b | acc << 2 | (in_acc == 0 ? 8u : 0u) | (flush ? 16u : 0u), 0);
+      const uint32_t ub = how & 3, uacc = how >> 2 & 1;
       if (elected) {
-        issue_chunk_mmas<false>(tmem_u + 128u * acc, tmem_u + 256 + 64 * b, tiles_u + b * 2 * TC_TILE_BYTES, 0, in_acc == 0);
-        mma_commit(done + 8 * b);
-        if (flush) mma_commit(d_full + 8 * acc);
+        issue_chunk_mmas<false>(tmem_u + 128u * uacc, tmem_u + 256 + 64 * ub, tiles_u + ub * 2 * TC_TILE_BYTES, 0, (how & 8) != 0);
+        mma_commit(done + 8 * ub);
+        if (how & 16) mma_commit(d_full + 8 * uacc);
       }
       __syncwarp();
       ++in_acc;

@@ -1473,7 +1473,7 @@ extern "C" int mb_experts_linear(const mb_experts* d, void* stream) {
   if ((rc = mb::weight_map(d->w_hi, d->n_in, d->n_in, &maps.hi, rows)) || (rc = mb::weight_map(d->w_lo, d->n_in, d->n_in, &maps.lo, rows))) return rc;
   const int shared = d->n_in == 128 ? 1 : 0;
   const int64_t items = ((d->n_slots + 127) / 128 + d->n_experts) * (shared ? 1 : d->n_out / 128);
-  mb::launch(mb::k_experts, (unsigned)(items < n_sm ? items : n_sm), mb::PS_THREADS, mb::EX_SMEM_BYTES, (cudaStream_t)stream, *d, maps, shared);
+  mb::launch(mb::k_experts, (unsigned)(items < n_sm ? items : n_sm), mb::EX_THREADS, mb::EX_SMEM_BYTES, (cudaStream_t)stream, *d, maps, shared);
   MB_LAUNCH_CHECK("k_experts");
   return MB_OK;
 }
