@@ -417,7 +417,7 @@ int mb_rmsnorm_bwd(int64_t n_rows, const float* x, const float* w, const float* 
  * [0, n_rows] are cut to it.  Rows of no segment are left as they are, or set to zero with zero_rest.  weight or bias NULL: 1, 0.
  * channels <= 1024, any row alignment (rows of 16-byte pieces take wide accesses); n_rows < 2^31.
  * bwd reads stats and writes dx and, where given, dweight and dbias [channels] (sums over all segments, in a fixed order).
- * scratch: mb_group_norm_scratch() bytes, 16-byte aligned, free again when the call's work is done. */
+ * scratch: mb_group_norm_scratch() bytes (0: NULL will do), 16-byte aligned, free again when the call's work is done. */
 typedef struct mb_group_norm {
   int64_t n_rows;
   int32_t n_seg, channels, groups, dtype, act, zero_rest; /* dtype of x, y, dy, dx; act: 0 none, 1 SiLU */
@@ -432,7 +432,7 @@ typedef struct mb_group_norm {
   float* dweight; float* dbias;
   void* scratch;
 } mb_group_norm;
-size_t mb_group_norm_scratch(int64_t n_rows, int32_t n_seg, int32_t channels);
+size_t mb_group_norm_scratch(int64_t n_rows, int32_t n_seg, int32_t channels, int32_t backward);
 int mb_group_norm_fwd(const mb_group_norm* d, void* stream);
 int mb_group_norm_bwd(const mb_group_norm* d, void* stream);
 
@@ -456,7 +456,7 @@ typedef struct mb_route {
   int32_t *offsets, *row_of, *slot_of;
   const float *dweights, *dloss;
   void* dlogits; int64_t ld_dlogits;
-  void* scratch;                                          /* fwd: mb_route_scratch() bytes */
+  void* scratch;                                          /* fwd: mb_route_scratch() bytes (0: NULL will do) */
 } mb_route;
 size_t mb_route_scratch(int64_t n_rows, int32_t n_experts);
 int mb_route_fwd(const mb_route* d, void* stream);

@@ -259,7 +259,7 @@ _OTHER = {
     "mb_status_string": (C.c_char_p, [C.c_int]),
     "mb_last_cuda_error": (C.c_char_p, []),
     "mb_graph_scan_tmp_len": (C.c_size_t, [_i64]),
-    "mb_group_norm_scratch": (C.c_size_t, [_i64, _i32, _i32]),
+    "mb_group_norm_scratch": (C.c_size_t, [_i64, _i32, _i32, _i32]),
     "mb_route_scratch": (C.c_size_t, [_i64, _i32]),
     "mb_experts_grad_scratch": (C.c_size_t, [_i64, _i32, _i32, _i32]),
 }

@@ -490,6 +490,8 @@ static int route_blocks(int64_t n_rows, int n_sm) {
   const int64_t most = 4 * (int64_t)n_sm, want = (n_rows + 63) / 64;
   return (int)(want < most ? (want > 0 ? want : 1) : most);
 }
+// few rows: one block does everything
+static bool route_small(int64_t n_rows, int n_experts) { return n_rows * n_experts <= 4096; }
 static bool route_valid(const mb_route* d) {
   return d && d->n_rows >= 0 && d->n_experts >= 1 && d->n_experts <= RT_MAX_EXPERTS && d->top_k >= 1 && d->top_k <= RT_MAX_K &&
          d->top_k <= d->n_experts && d->dtype >= 0 && d->dtype <= 2 && d->n_rows * d->top_k <= INT32_MAX;
@@ -543,15 +545,17 @@ using namespace mb;
 
 extern "C" size_t mb_route_scratch(int64_t n_rows, int32_t n_experts) {
   int n_sm = 0;
-  if (n_rows < 0 || n_experts < 1 || sm_count(&n_sm) != MB_OK) return 0;
+  if (n_rows < 0 || n_experts < 1 || route_small(n_rows, n_experts) || sm_count(&n_sm) != MB_OK) return 0;
   const size_t nb = (size_t)route_blocks(n_rows, n_sm);
   return 8 * (size_t)n_experts + 4 * nb * (2 * (size_t)n_experts + 1);
 }
 
 extern "C" int mb_route_fwd(const mb_route* d, void* stream) {
   if (!route_valid(d) || !d->counts || !d->loss || !d->offsets) return MB_ERR_INVALID;
-  if (d->n_rows > 0 && (!d->logits || d->ld_logits < d->n_experts || !d->ids || !d->weights || !d->row_of || !d->slot_of || !d->scratch))
+  if (d->n_rows > 0 && (!d->logits || d->ld_logits < d->n_experts || !d->ids || !d->weights || !d->row_of || !d->slot_of))
     return MB_ERR_INVALID;
+  const bool small = route_small(d->n_rows, d->n_experts);
+  if (!small && !d->scratch) return MB_ERR_INVALID;
   const cudaStream_t st = (cudaStream_t)stream;
   int n_sm = 0, rc = sm_count(&n_sm);
   if (rc) return rc;
@@ -561,7 +565,6 @@ extern "C" int mb_route_fwd(const mb_route* d, void* stream) {
   a.p_total = static_cast<double*>(d->scratch);
   a.p_part = reinterpret_cast<float*>(a.p_total + d->n_experts);
   a.c_part = reinterpret_cast<int32_t*>(a.p_part + (size_t)d->n_experts * a.n_blocks);
-  const bool small = d->n_rows * (int64_t)d->n_experts <= 4096;
   route_typed(d->dtype, route_vector(d, d->logits, d->ld_logits), d->n_experts, RouteFwd{a, st, small});
   if (!small) {
     launch(k_route_scan, (unsigned)cdiv(d->n_experts + 1, RT_WARPS), RT_THREADS, 0, st, a);

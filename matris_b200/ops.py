@@ -449,49 +449,88 @@ def segment_sum_scalar(n_seg, seg_ptr, x):
 
 
 # ------------------------------------------------------------------ group norm and mixture of experts
+# These calls serve single structures and single rows too, where the host's share counts: shapes are compared as tuples, outputs
+# that live together share an allocation, descriptors are packed with one struct call (layouts checked against ctypes below).
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_F32, _I32 = torch.float32, torch.int32
+_NORM_FMT = struct.Struct("<q6ifi" + "QQqQQQqQ" + "QqQq" + "QQQ")
+_ROUTE_FMT = struct.Struct("<q4i" + "QqQQQQQ" + "QQQ" + "QQ" + "QqQ")
+_EXPERTS_FMT = struct.Struct("<qq6i" + "QQ" + "Qq" + "QQQ" + "Qq" * 3 + "QQQ")
+_COMBINE_FMT = struct.Struct("<qq4i" + "QQQ" + "Qq" * 4 + "Q")
+assert [f.size for f in (_NORM_FMT, _ROUTE_FMT, _EXPERTS_FMT, _COMBINE_FMT)] == [
+    C.sizeof(t) for t in (_lib.MbGroupNorm, _lib.MbRoute, _lib.MbExperts, _lib.MbCombine)]
+_cuda_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _take(t, name, dtype, shape=None, dense=True):
-    """Check one argument: element type, shape (None: any size), layout.  The device is checked last (``_here``)."""
+def _take(t, name, dtype, shape):
+    """Check a contiguous argument of a given element type and shape.  The device is checked last (``_here``)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: a tensor is wanted, got {type(t).__name__}")
-    if t.dtype not in (dtype if isinstance(dtype, (tuple, dict)) else (dtype,)):
-        raise TypeError(f"{name}: element type {t.dtype}")
-    if shape is not None and (t.dim() != len(shape) or any(w is not None and w != h for w, h in zip(shape, t.shape))):
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, {tuple('any' if w is None else w for w in shape)} is wanted")
-    if dense and not t.is_contiguous():
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: element type {t.dtype}, {dtype} is wanted")
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, {shape} is wanted")
+    if not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous tensor is wanted, got strides {t.stride()}")
     return t
 
 
-def _row_stride(t, name):
-    """Row stride of a [rows, width] tensor whose rows are contiguous and do not overlap."""
-    if t.shape[1] > 1 and t.stride(1) != 1:
+def _take_vector(t, name):
+    """Check a contiguous int32 vector; its length."""
+    if not isinstance(t, torch.Tensor) or t.dtype != _I32:
+        raise TypeError(f"{name}: an int32 tensor is wanted, got {getattr(t, 'dtype', type(t).__name__)}")
+    if t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous vector is wanted, got shape {tuple(t.shape)}, strides {t.stride()}")
+    return t.shape[0]
+
+
+def _take_rows(t, name, dtype, n=None, width=None, aligned=False):
+    """Check a [rows, width] argument whose rows are contiguous and do not overlap (``aligned``: and start on 16-byte
+    boundaries, for kernels that read them in such pieces); its row stride."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a tensor is wanted, got {type(t).__name__}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: element type {t.dtype}, {dtype} is wanted")
+    shape = t.shape
+    if len(shape) != 2 or (n is not None and shape[0] != n) or (width is not None and shape[1] != width):
+        raise ValueError(f"{name}: shape {tuple(shape)}, ({'rows' if n is None else n}, {'width' if width is None else width}) is wanted")
+    rows, cols = shape
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
         raise ValueError(f"{name}: the values of a row have to be neighbours, got strides {t.stride()}")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+    if rows <= 1:
+        ld = cols
+    elif ld < cols:
         raise ValueError(f"{name}: rows overlap, got strides {t.stride()}")
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
-
-
-def _aligned_rows(t, name):
-    """``_row_stride`` of rows that are read in 16-byte pieces."""
-    ld = _row_stride(t, name)
-    if t.data_ptr() % 16 or (t.shape[0] > 1 and ld * t.element_size() % 16):
+    if aligned and (t.data_ptr() % 16 or (rows > 1 and ld * t.element_size() % 16)):
         raise ValueError(f"{name}: rows have to start on 16-byte boundaries")
     return ld
 
 
-def _here(**tensors):
-    """The launches go to the current device: every tensor has to be there."""
-    for name, t in tensors.items():
-        if t is not None and (t.device.type != "cuda" or t.device.index != torch.cuda.current_device()):
-            raise ValueError(f"{name} is on {t.device}: it has to be on the current CUDA device")
+def _here(*tensors):
+    """The launches go to the current device: every tensor has to be there.  Returns its number."""
+    if not all([t is None or t.is_cuda for t in tensors]):
+        raise ValueError(f"tensors on the CPU ({[str(t.device) for t in tensors if t is not None]}): they have to be on the current CUDA device")
+    device = _cuda_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"a tensor on {t.device}: it has to be on the current CUDA device, cuda:{device}")
+    return device
+
+
+def _launch(name, struct_type, data, device):
+    d = struct_type.from_buffer_copy(data)
+    call(name, C.byref(d), _stream() if _raw_stream is None else _raw_stream(device))
+
+
+def _scratch(size, like):
+    return torch.empty(size, dtype=torch.uint8, device=like.device) if size else None
 
 
 def _norm_rows(x, weight, bias, seg_ptr, n_groups, act, eps):
-    """[rows, channels] view, row stride and number of segments of a group norm's input."""
-    _take(x, "x", _DTYPES, dense=False)
+    """Rows (a [rows, channels] view), channels, row stride and number of segments of a group norm's input."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPES:
+        raise TypeError(f"x: a float32, bfloat16 or float16 tensor is wanted, got {getattr(x, 'dtype', type(x).__name__)}")
     if seg_ptr is None:
         if x.dim() < 2:
             raise ValueError("x: [batch, .., channels] is wanted without seg_ptr")
@@ -499,42 +538,35 @@ def _norm_rows(x, weight, bias, seg_ptr, n_groups, act, eps):
             raise ValueError(f"x: a contiguous tensor is wanted without seg_ptr, got strides {x.stride()}")
         n_seg, x = x.shape[0], x.view(math.prod(x.shape[:-1]), x.shape[-1])
     else:
-        _take(x, "x", _DTYPES, (None, None), dense=False)
-        n_seg = _take(seg_ptr, "seg_ptr", torch.int32, (None,)).shape[0] - 1
+        n_seg = _take_vector(seg_ptr, "seg_ptr") - 1
         if n_seg < 0:
             raise ValueError("seg_ptr: [segments + 1] offsets are wanted, got none")
-    channels = x.shape[1]
+    ld = _take_rows(x, "x", x.dtype)
+    rows, channels = x.shape
     if not 1 <= channels <= 1024:
         raise NotImplementedError(f"group norm takes 1 to 1024 channels, got {channels}")
     if n_groups < 1 or channels % n_groups:
         raise ValueError(f"{channels} channels do not divide into {n_groups} groups")
-    if act not in (0, 1):
+    if act != 0 and act != 1:
         raise ValueError(f"act={act!r}: 0 (none) or 1 (SiLU)")
     if not eps > 0:
         raise ValueError(f"eps={eps!r} has to be positive")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _take(t, name, torch.float32, (channels,))
-    _row_stride(x, "x")
-    if x.shape[0] >= 1 << 31:
+    if weight is not None:
+        _take(weight, "weight", _F32, (channels,))
+    if bias is not None:
+        _take(bias, "bias", _F32, (channels,))
+    if rows >= 1 << 31:
         raise NotImplementedError("group norm takes fewer than 2**31 rows")
-    return x, n_seg
+    return x, rows, channels, ld, n_seg
 
 
-def _norm_desc(x, weight, bias, n_groups, n_seg, seg_ptr, eps, act, stats):
-    d = _lib.MbGroupNorm()
-    d.n_rows, d.n_seg, d.channels, d.groups = x.shape[0], n_seg, x.shape[1], n_groups
-    d.dtype, d.act, d.eps = _DTYPES[x.dtype], act, eps
-    d.weight, d.bias, d.seg_ptr, d.x, d.ld_x, d.stats = ptr(weight), ptr(bias), ptr(seg_ptr), ptr(x), _row_stride(x, "x"), ptr(stats)
-    return d
-
-
-def _norm_out(x, x_given, out, name):
-    """The output rows (same shape and type as the input) and whether rows of no segment are to be cleared."""
+def _norm_out(like, rows, channels, out, seg_ptr):
+    """The output, its row stride, and whether rows of no segment are to be cleared."""
     if out is None:
-        return torch.empty(x_given.shape, dtype=x.dtype, device=x.device), True
-    _take(out, name, x.dtype, tuple(x_given.shape), dense=x_given.dim() != 2)
-    return out, False
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device), channels, 1
+    if seg_ptr is None:
+        return _take(out, "out", like.dtype, like.shape), channels, 0
+    return out, _take_rows(out, "out", like.dtype, rows, channels), 0
 
 
 def group_norm_fwd(x, weight, bias, n_groups, seg_ptr=None, eps=1e-5, act=0, out=None):
@@ -544,41 +576,43 @@ def group_norm_fwd(x, weight, bias, n_groups, seg_ptr=None, eps=1e-5, act=0, out
     ``x`` [rows, channels] with ``seg_ptr`` (int32 [segments + 1] row offsets on the device, as a batch's ``atom_ptr``), or
     [batch, .., channels] without.  Returns (y, stats): stats [segments, groups, 2] (mean, 1 / deviation) is what
     ``group_norm_bwd`` reads.  Rows of no segment are zero in a returned tensor and left alone in a given ``out``, which may be x."""
-    rows, n_seg = _norm_rows(x, weight, bias, seg_ptr, n_groups, act, eps)
-    y, zero = _norm_out(rows, x, out, "out")
-    _here(x=x, weight=weight, bias=bias, seg_ptr=seg_ptr, out=out)
-    if zero and n_seg == 0:
+    xr, rows, channels, ld, n_seg = _norm_rows(x, weight, bias, seg_ptr, n_groups, act, eps)
+    device = _here(x, weight, bias, seg_ptr, out)
+    y, ld_y, zero = _norm_out(x, rows, channels, out, seg_ptr)
+    stats = torch.empty((n_seg, n_groups, 2), dtype=_F32, device=x.device)
+    if not rows:
+        stats.zero_()
+    if zero and not n_seg:
         y.zero_()
-    stats = new(n_seg * n_groups, 2, x, zero=not rows.shape[0]).view(n_seg, n_groups, 2)
-    d = _norm_desc(rows, weight, bias, n_groups, n_seg, seg_ptr, eps, act, stats)
-    yr = y if seg_ptr is not None else y.view(rows.shape)
-    d.y, d.ld_y, d.zero_rest = ptr(yr), _row_stride(yr, "out"), int(zero)
-    scratch = torch.empty(_lib.load().mb_group_norm_scratch(d.n_rows, n_seg, d.channels), dtype=torch.uint8, device=x.device)
-    d.scratch = ptr(scratch)
-    call("mb_group_norm_fwd", C.byref(d), _stream())
+    scratch = _scratch(_lib.load().mb_group_norm_scratch(rows, n_seg, channels, 0), x)
+    _launch("mb_group_norm_fwd", _lib.MbGroupNorm, _NORM_FMT.pack(
+        rows, n_seg, channels, n_groups, _DTYPES[x.dtype], act, zero, eps, 0, ptr(seg_ptr) or 0, xr.data_ptr(), ld, ptr(weight) or 0,
+        ptr(bias) or 0, y.data_ptr(), ld_y, stats.data_ptr(), 0, 0, 0, 0, 0, 0, ptr(scratch) or 0), device)
     return y, stats
 
 
 def group_norm_bwd(dy, x, weight, bias, stats, n_groups, seg_ptr=None, act=0, out=None, want_affine=True):
     """Gradients (dx, dweight, dbias) of ``group_norm_fwd`` from its inputs and ``stats``; dweight and dbias are None unless
     ``want_affine``.  dx is written to ``out`` where given (it may be dy or x)."""
-    rows, n_seg = _norm_rows(x, weight, bias, seg_ptr, n_groups, act, 1.0)
-    _take(dy, "dy", x.dtype, tuple(x.shape), dense=seg_ptr is None)
-    _take(stats, "stats", torch.float32, (n_seg, n_groups, 2))
-    dx, zero = _norm_out(rows, x, out, "out")
-    _here(x=x, dy=dy, weight=weight, bias=bias, stats=stats, seg_ptr=seg_ptr, out=out)
-    if zero and n_seg == 0:
+    xr, rows, channels, ld, n_seg = _norm_rows(x, weight, bias, seg_ptr, n_groups, act, 1.0)
+    if seg_ptr is None:
+        _take(dy, "dy", x.dtype, x.shape)
+        ld_dy = channels
+    else:
+        ld_dy = _take_rows(dy, "dy", x.dtype, rows, channels)
+    _take(stats, "stats", _F32, (n_seg, n_groups, 2))
+    device = _here(x, dy, weight, bias, stats, seg_ptr, out)
+    dx, ld_dx, zero = _norm_out(x, rows, channels, out, seg_ptr)
+    if zero and not n_seg:
         dx.zero_()
-    d = _norm_desc(rows, weight, bias, n_groups, n_seg, seg_ptr, 1.0, act, stats)
-    dyr, dxr = (dy, dx) if seg_ptr is not None else (dy.view(rows.shape), dx.view(rows.shape))
-    d.dy, d.ld_dy, d.dx, d.ld_dx, d.zero_rest = ptr(dyr), _row_stride(dyr, "dy"), ptr(dxr), _row_stride(dxr, "out"), int(zero)
     dweight = dbias = None
     if want_affine:
-        dweight, dbias = torch.empty(2, d.channels, dtype=torch.float32, device=x.device).unbind(0)
-        d.dweight, d.dbias = ptr(dweight), ptr(dbias)
-    scratch = torch.empty(_lib.load().mb_group_norm_scratch(d.n_rows, n_seg, d.channels), dtype=torch.uint8, device=x.device)
-    d.scratch = ptr(scratch)
-    call("mb_group_norm_bwd", C.byref(d), _stream())
+        dweight, dbias = torch.empty((2, channels), dtype=_F32, device=x.device).unbind(0)
+    scratch = _scratch(_lib.load().mb_group_norm_scratch(rows, n_seg, channels, 1), x)
+    _launch("mb_group_norm_bwd", _lib.MbGroupNorm, _NORM_FMT.pack(
+        rows, n_seg, channels, n_groups, _DTYPES[x.dtype], act, zero, 1.0, 0, ptr(seg_ptr) or 0, xr.data_ptr(), ld, ptr(weight) or 0,
+        ptr(bias) or 0, 0, 0, stats.data_ptr(), dy.data_ptr(), ld_dy, dx.data_ptr(), ld_dx, ptr(dweight) or 0, ptr(dbias) or 0,
+        ptr(scratch) or 0), device)
     return dx, dweight, dbias
 
 
@@ -600,8 +634,11 @@ class Route(NamedTuple):
         return self.totals[:-1]
 
 
-def _route_desc(logits, top_k, renorm):
-    _take(logits, "logits", _DTYPES, (None, None), dense=False)
+def _route_args(logits, top_k):
+    """Row stride, rows and experts of the router's logits."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES:
+        raise TypeError(f"logits: a float32, bfloat16 or float16 tensor is wanted, got {getattr(logits, 'dtype', type(logits).__name__)}")
+    ld = _take_rows(logits, "logits", logits.dtype)
     n, n_experts = logits.shape
     if not 1 <= n_experts <= 1024:
         raise NotImplementedError(f"the router takes 1 to 1024 experts, got {n_experts}")
@@ -609,10 +646,7 @@ def _route_desc(logits, top_k, renorm):
         raise ValueError(f"top_k={top_k}: 1 to {min(32, n_experts)} of {n_experts} experts")
     if n * top_k >= 1 << 31:
         raise NotImplementedError("the router takes fewer than 2**31 choices")
-    d = _lib.MbRoute()
-    d.n_rows, d.n_experts, d.top_k, d.dtype, d.renorm = n, n_experts, top_k, _DTYPES[logits.dtype], int(renorm)
-    d.logits, d.ld_logits = ptr(logits), _row_stride(logits, "logits")
-    return d
+    return ld, n, n_experts
 
 
 def route_fwd(logits, top_k, valid=None, renorm=True) -> Route:
@@ -623,39 +657,43 @@ def route_fwd(logits, top_k, valid=None, renorm=True) -> Route:
     loss = experts / (top_k T^2) sum_e counts_e sum_rows p_e with T the rows routed: 1 where both are even.  Slots 0, 1, ..
     hold the pairs in order of expert, then of row: expert e has slots offsets[e] .. offsets[e+1] - 1, slot s is of row row_of[s]
     (-1 behind the last), choice j of row t has slot slot_of[t, j]."""
-    d = _route_desc(logits, top_k, renorm)
-    n, n_experts = logits.shape
+    ld, n, n_experts = _route_args(logits, top_k)
     if valid is not None:
         _take(valid, "valid", torch.bool, (n,))
-    _here(logits=logits, valid=valid)
-    dev = logits.device
-    ints = torch.empty(2 * n_experts + 2, dtype=torch.int32, device=dev)
-    ids, slot_of, row_of = torch.empty(3, n * top_k, dtype=torch.int32, device=dev).unbind(0)
-    weights, loss = torch.empty(n, top_k, dtype=torch.float32, device=dev), torch.empty((), dtype=torch.float32, device=dev)
-    totals, offsets = ints[:n_experts + 1], ints[n_experts + 1:]
-    scratch = torch.empty(_lib.load().mb_route_scratch(n, n_experts), dtype=torch.uint8, device=dev)
-    d.valid, d.ids, d.weights, d.counts, d.loss = ptr(valid), ptr(ids), ptr(weights), ptr(totals), ptr(loss)
-    d.offsets, d.row_of, d.slot_of, d.scratch = ptr(offsets), ptr(row_of), ptr(slot_of), ptr(scratch)
-    call("mb_route_fwd", C.byref(d), _stream())
-    return Route(ids.view(n, top_k), weights, loss, totals, offsets, row_of, slot_of.view(n, top_k), bool(renorm))
+    device = _here(logits, valid)
+    renorm, pairs = bool(renorm), n * top_k
+    dev, shape = logits.device, (n, top_k)
+    block = torch.empty(2 * n_experts + 2 + pairs, dtype=_I32, device=dev)
+    totals, offsets, row_of = torch.split_with_sizes(block, (n_experts + 1, n_experts + 1, pairs))
+    ids, slot_of = torch.empty((2, *shape), dtype=_I32, device=dev).unbind(0)
+    weights, loss = torch.empty(shape, dtype=_F32, device=dev), torch.empty((), dtype=_F32, device=dev)
+    scratch = _scratch(_lib.load().mb_route_scratch(n, n_experts), logits)
+    _launch("mb_route_fwd", _lib.MbRoute, _ROUTE_FMT.pack(
+        n, n_experts, top_k, _DTYPES[logits.dtype], renorm, logits.data_ptr(), ld, ptr(valid) or 0, ids.data_ptr(), weights.data_ptr(),
+        totals.data_ptr(), loss.data_ptr(), offsets.data_ptr(), row_of.data_ptr(), slot_of.data_ptr(), 0, 0, 0, 0, ptr(scratch) or 0), device)
+    return Route(ids, weights, loss, totals, offsets, row_of, slot_of, renorm)
 
 
 def route_bwd(logits, route: Route, dweights=None, dloss=None):
     """Gradient of the logits from those of the weights [rows, top_k] and of the balance loss (a scalar tensor); None: zero."""
-    n, top_k = route.ids.shape
-    d = _route_desc(logits, top_k, route.renorm)
-    _take(route.ids, "route.ids", torch.int32, (logits.shape[0], top_k))
-    _take(route.weights, "route.weights", torch.float32, (n, top_k))
-    _take(route.totals, "route.totals", torch.int32, (logits.shape[1] + 1,))
+    ids = route.ids
+    if ids.dim() != 2:
+        raise ValueError(f"route.ids: [rows, top_k] is wanted, got shape {tuple(ids.shape)}")
+    top_k = ids.shape[1]
+    ld, n, n_experts = _route_args(logits, top_k)
+    shape = (n, top_k)
+    _take(ids, "route.ids", _I32, shape)
+    _take(route.weights, "route.weights", _F32, shape)
+    _take(route.totals, "route.totals", _I32, (n_experts + 1,))
     if dweights is not None:
-        _take(dweights, "dweights", torch.float32, (n, top_k))
-    if dloss is not None and _take(dloss, "dloss", torch.float32).numel() != 1:
-        raise ValueError(f"dloss: a scalar is wanted, got shape {tuple(dloss.shape)}")
-    _here(logits=logits, ids=route.ids, weights=route.weights, totals=route.totals, dweights=dweights, dloss=dloss)
-    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    d.ids, d.weights, d.counts, d.dweights, d.dloss = ptr(route.ids), ptr(route.weights), ptr(route.totals), ptr(dweights), ptr(dloss)
-    d.dlogits, d.ld_dlogits = ptr(dlogits), logits.shape[1]
-    call("mb_route_bwd", C.byref(d), _stream())
+        _take(dweights, "dweights", _F32, shape)
+    if dloss is not None and (dloss.dtype != _F32 or dloss.numel() != 1):
+        raise ValueError(f"dloss: a float32 scalar is wanted, got {dloss.dtype}, shape {tuple(dloss.shape)}")
+    device = _here(logits, ids, route.weights, route.totals, dweights, dloss)
+    dlogits = torch.empty((n, n_experts), dtype=logits.dtype, device=logits.device)
+    _launch("mb_route_bwd", _lib.MbRoute, _ROUTE_FMT.pack(
+        n, n_experts, top_k, _DTYPES[logits.dtype], route.renorm, logits.data_ptr(), ld, 0, ids.data_ptr(), route.weights.data_ptr(),
+        route.totals.data_ptr(), 0, 0, 0, 0, ptr(dweights) or 0, ptr(dloss) or 0, dlogits.data_ptr(), n_experts, 0), device)
     return dlogits
 
 
@@ -663,16 +701,22 @@ class ExpertWeights:
     """Weights [experts, n_out, n_in] of the experts' dense layers, laid out once for ``experts_linear`` in both directions:
     two tf32 parts each, w = hi + lo to 2^-23, 16 bytes a weight.  It copies: a later change of ``w`` does not reach it."""
 
-    __slots__ = ("shape", "parts")
+    __slots__ = ("shape", "parts", "ptrs")
 
     def __init__(self, w: torch.Tensor):
-        w = _take(w.detach(), "weights", torch.float32, (None, None, None), dense=False).contiguous()
+        if not isinstance(w, torch.Tensor) or w.dtype != _F32:
+            raise TypeError(f"weights: a float32 tensor is wanted, got {getattr(w, 'dtype', type(w).__name__)}")
+        if w.dim() != 3:
+            raise ValueError(f"weights: [experts, n_out, n_in] is wanted, got shape {tuple(w.shape)}")
         if not 1 <= w.shape[0] <= 1024:
             raise NotImplementedError(f"1 to 1024 experts, got {w.shape[0]}")
         _expert_widths(w.shape[2], w.shape[1])
-        _here(weights=w)
-        self.shape, self.parts = tuple(w.shape), new(4, w.numel(), w)
-        call("mb_experts_split", *self.shape, ptr(w), ptr(self.parts), _stream())
+        device = _here(w)
+        w = w.detach().contiguous()
+        self.shape, self.parts = tuple(w.shape), torch.empty((4, w.numel()), dtype=_F32, device=w.device)
+        first, step = self.parts.data_ptr(), 4 * w.numel()
+        self.ptrs = tuple(first + i * step for i in range(4))  # hi, lo, hi and lo of the transposes
+        call("mb_experts_split", *self.shape, w.data_ptr(), first, _stream() if _raw_stream is None else _raw_stream(device))
 
 
 def _expert_widths(n_in, n_out):
@@ -681,22 +725,19 @@ def _expert_widths(n_in, n_out):
             raise NotImplementedError(f"the experts' kernels take widths 128, 256 .. 1024, got {n_in} -> {n_out}")
 
 
-def _experts_desc(x, offsets, idx, n_in, n_out, in_act):
-    _take(x, "x", torch.float32, (None, n_in), dense=False)
-    _take(offsets, "offsets", torch.int32, (None,))
-    d = _lib.MbExperts()
-    d.n_rows = d.n_slots = x.shape[0]
+def _expert_rows(x, idx, n_in, in_act):
+    """Row stride and number of rows of an experts' input, and its number of slots."""
+    ld = _take_rows(x, "x", _F32, width=n_in, aligned=True)
+    n_rows = n_slots = x.shape[0]
     if idx is not None:
-        d.n_slots = _take(idx, "idx", torch.int32, (None,)).shape[0]
-        if d.n_slots and not d.n_rows:
+        n_slots = _take_vector(idx, "idx")
+        if n_slots and not n_rows:
             raise ValueError("idx: there are no rows to take")
-    if d.n_slots >= 1 << 31:
-        raise NotImplementedError("fewer than 2**31 slots")
-    if in_act not in (0, 1):
+    if n_slots >= 1 << 31 or n_rows >= 1 << 31:
+        raise NotImplementedError("fewer than 2**31 rows and slots")
+    if in_act != 0 and in_act != 1:
         raise ValueError(f"in_act={in_act!r}: 0 (none) or 1 (SiLU)")
-    d.n_experts, d.n_in, d.n_out, d.in_act = offsets.shape[0] - 1, n_in, n_out, in_act
-    d.offsets, d.idx, d.x, d.ld_x = ptr(offsets), ptr(idx), ptr(x), _aligned_rows(x, "x")
-    return d
+    return ld, n_rows, n_slots
 
 
 def experts_linear(x, weights, offsets, bias=None, idx=None, in_act=0, out_act=0, gate=None, transposed=False, out=None):
@@ -705,96 +746,98 @@ def experts_linear(x, weights, offsets, bias=None, idx=None, in_act=0, out_act=0
 
     ``weights``: ExpertWeights, or a [experts, n_out, n_in] tensor that is laid out in the call; ``transposed``: W_e in the place
     of its transpose, the data gradient.  ``in_act`` / ``out_act`` 1: SiLU.  ``offsets``, ``idx``: ``Route.offsets``, ``Route.row_of``.
-    Slots behind the last are zero in a returned tensor and left alone in a given ``out``."""
+    Slots behind the last are zero in a returned tensor and left alone in a given ``out``, which must not overlap the inputs."""
     if not isinstance(weights, ExpertWeights):
         weights = ExpertWeights(weights)
     n_experts, n_out, n_in = weights.shape
-    w_hi = ptr(weights.parts) + (8 * weights.parts.shape[1] if transposed else 0)
+    w_hi, w_lo = weights.ptrs[:2]
     if transposed:
         n_out, n_in = n_in, n_out
-    d = _experts_desc(x, offsets, idx, n_in, n_out, in_act)
-    if d.n_experts != n_experts:
+        w_hi, w_lo = weights.ptrs[2:]
+    ld, n_rows, n_slots = _expert_rows(x, idx, n_in, in_act)
+    if _take_vector(offsets, "offsets") != n_experts + 1:
         raise ValueError(f"offsets: [{n_experts + 1}] is wanted, got {tuple(offsets.shape)}")
-    if out_act not in (0, 1):
+    if out_act != 0 and out_act != 1:
         raise ValueError(f"out_act={out_act!r}: 0 (none) or 1 (SiLU)")
     if bias is not None:
-        _take(bias, "bias", torch.float32, (n_experts, n_out))
-    if gate is not None:
-        _take(gate, "gate", torch.float32, (d.n_slots, n_out), dense=False)
-        d.gate, d.ld_gate = ptr(gate), _aligned_rows(gate, "gate")
-    if out is not None:
-        _take(out, "out", torch.float32, (d.n_slots, n_out), dense=False)
-    _here(x=x, weights=weights.parts, offsets=offsets, bias=bias, idx=idx, gate=gate, out=out)
-    y = new(d.n_slots, n_out, x) if out is None else out
-    d.w_hi, d.w_lo = w_hi, w_hi + 4 * weights.parts.shape[1]
-    d.bias, d.out_act, d.zero_rest = ptr(bias), out_act, int(out is None)
-    d.y, d.ld_y = ptr(y), _aligned_rows(y, "out")
-    call("mb_experts_linear", C.byref(d), _stream())
+        _take(bias, "bias", _F32, (n_experts, n_out))
+        if bias.data_ptr() % 16:
+            raise ValueError("bias has to start on a 16-byte boundary")
+    ld_gate = 0 if gate is None else _take_rows(gate, "gate", _F32, n_slots, n_out, aligned=True)
+    ld_y = n_out if out is None else _take_rows(out, "out", _F32, n_slots, n_out, aligned=True)
+    device = _here(x, weights.parts, offsets, bias, idx, gate, out)
+    y = torch.empty((n_slots, n_out), dtype=_F32, device=x.device) if out is None else out
+    _launch("mb_experts_linear", _lib.MbExperts, _EXPERTS_FMT.pack(
+        n_slots, n_rows, n_experts, n_in, n_out, in_act, out_act, out is None, offsets.data_ptr(), ptr(idx) or 0, x.data_ptr(), ld, w_hi, w_lo,
+        ptr(bias) or 0, ptr(gate) or 0, ld_gate, y.data_ptr(), ld_y, 0, 0, 0, 0, 0), device)
     return y
 
 
 def experts_grad_w(dy, x, offsets, idx=None, in_act=0, want_bias=True):
     """Weight gradients of ``experts_linear``: (dW [experts, n_out, n_in], dbias [experts, n_out] or None) with
     dW_e = sum over the slots of e of dy[s]^T f(x[idx[s]]), summed in a fixed order.  An expert without slots has zeros."""
-    _take(dy, "dy", torch.float32, (None, None), dense=False)
-    if x.dim() != 2:
-        raise ValueError(f"x: [rows, n_in] is wanted, got shape {tuple(x.shape)}")
-    _expert_widths(x.shape[1], dy.shape[1])
-    d = _experts_desc(x, offsets, idx, x.shape[1], dy.shape[1], in_act)
-    if dy.shape[0] != d.n_slots:
-        raise ValueError(f"dy: {d.n_slots} slots are wanted, got {dy.shape[0]}")
-    if not 1 <= d.n_experts <= 1024:
-        raise NotImplementedError(f"1 to 1024 experts, got {d.n_experts}")
-    d.dy, d.ld_dy = ptr(dy), _aligned_rows(dy, "dy")
-    _here(dy=dy, x=x, offsets=offsets, idx=idx)
-    dw = torch.empty(d.n_experts, d.n_out, d.n_in, dtype=torch.float32, device=x.device)
-    dbias = torch.empty(d.n_experts, d.n_out, dtype=torch.float32, device=x.device) if want_bias else None
-    scratch = torch.empty(_lib.load().mb_experts_grad_scratch(d.n_slots, d.n_experts, d.n_in, d.n_out), dtype=torch.uint8, device=x.device)
-    d.dw, d.dbias, d.scratch = ptr(dw), ptr(dbias), ptr(scratch)
-    call("mb_experts_grad_w", C.byref(d), _stream())
+    ld, n_rows, n_slots = _expert_rows(x, idx, None, in_act)
+    ld_dy = _take_rows(dy, "dy", _F32, n_slots, aligned=True)
+    n_in, n_out = x.shape[1], dy.shape[1]
+    _expert_widths(n_in, n_out)
+    n_experts = _take_vector(offsets, "offsets") - 1
+    if not 1 <= n_experts <= 1024:
+        raise NotImplementedError(f"1 to 1024 experts, got {n_experts}")
+    device = _here(dy, x, offsets, idx)
+    dw = torch.empty((n_experts, n_out, n_in), dtype=_F32, device=x.device)
+    dbias = torch.empty((n_experts, n_out), dtype=_F32, device=x.device) if want_bias else None
+    scratch = _scratch(_lib.load().mb_experts_grad_scratch(n_slots, n_experts, n_in, n_out), x)
+    _launch("mb_experts_grad_w", _lib.MbExperts, _EXPERTS_FMT.pack(
+        n_slots, n_rows, n_experts, n_in, n_out, in_act, 0, 0, offsets.data_ptr(), ptr(idx) or 0, x.data_ptr(), ld, 0, 0, 0, 0, 0, 0, 0,
+        dy.data_ptr(), ld_dy, dw.data_ptr(), ptr(dbias) or 0, ptr(scratch) or 0), device)
     return dw, dbias
 
 
-def _combine_desc(y, slot_of, weights):
-    _take(y, "y", torch.float32, (None, None), dense=False)
-    n, k = _take(slot_of, "slot_of", torch.int32, (None, None)).shape
-    if y.shape[1] % 4 or not y.shape[1]:
-        raise NotImplementedError(f"widths that are multiples of 4, got {y.shape[1]}")
-    if k < 1 or n * k >= 1 << 31 or y.shape[0] >= 1 << 31:
+def _combine_args(y, slot_of, weights):
+    """Row stride and shape of the experts' outputs, rows and choices a row."""
+    if y.dim() != 2:
+        raise ValueError(f"y: [slots, width] is wanted, got shape {tuple(y.shape)}")
+    if not isinstance(slot_of, torch.Tensor) or slot_of.dtype != _I32:
+        raise TypeError(f"slot_of: an int32 tensor is wanted, got {getattr(slot_of, 'dtype', type(slot_of).__name__)}")
+    if slot_of.dim() != 2 or not slot_of.is_contiguous():
+        raise ValueError(f"slot_of: contiguous [rows, top_k] is wanted, got shape {tuple(slot_of.shape)}, strides {slot_of.stride()}")
+    (n_slots, width), (n, k) = y.shape, slot_of.shape
+    if width % 4 or not width:
+        raise NotImplementedError(f"widths that are multiples of 4, got {width}")
+    if k < 1 or n * k >= 1 << 31 or n_slots >= 1 << 31:
         raise NotImplementedError(f"1 choice a row or more, fewer than 2**31 in all, got {n} x {k}")
+    ld = _take_rows(y, "y", _F32, aligned=True)
     if weights is not None:
-        _take(weights, "weights", torch.float32, (n, k))
-    d = _lib.MbCombine()
-    d.n_rows, d.n_slots, d.top_k, d.width = n, y.shape[0], k, y.shape[1]
-    d.slot_of, d.weights, d.y, d.ld_y = ptr(slot_of), ptr(weights), ptr(y), _aligned_rows(y, "y")
-    return d
+        _take(weights, "weights", _F32, (n, k))
+    return ld, n_slots, width, n, k
 
 
 def experts_combine_fwd(y, slot_of, weights=None):
     """The experts' outputs back to their rows: out[t] = sum_j weights[t, j] y[slot_of[t, j]] over the choices with a slot
     (weights None: 1, the sum that the gradient of the gathered rows takes)."""
-    d = _combine_desc(y, slot_of, weights)
-    _here(y=y, slot_of=slot_of, weights=weights)
-    out = new(d.n_rows, d.width, y)
-    d.out, d.ld_out = ptr(out), d.width
-    call("mb_experts_combine_fwd", C.byref(d), _stream())
+    ld, n_slots, width, n, k = _combine_args(y, slot_of, weights)
+    device = _here(y, slot_of, weights)
+    out = torch.empty((n, width), dtype=_F32, device=y.device)
+    _launch("mb_experts_combine_fwd", _lib.MbCombine, _COMBINE_FMT.pack(
+        n, n_slots, k, width, 0, 0, slot_of.data_ptr(), 0, ptr(weights) or 0, y.data_ptr(), ld, out.data_ptr(), width, 0, 0, 0, 0, 0), device)
     return out
 
 
 def experts_combine_bwd(dout, y, slot_of, weights=None, offsets=None):
     """Gradients (dy, dweights) of ``experts_combine_fwd``: dy [slots, width], dweights [rows, top_k] (0 for a choice without a
     slot).  Slots that no choice has are zero from ``offsets[-1]`` on; without ``offsets`` every slot has to have its choice."""
-    d = _combine_desc(y, slot_of, weights)
-    _take(dout, "dout", torch.float32, (d.n_rows, d.width), dense=False)
+    ld, n_slots, width, n, k = _combine_args(y, slot_of, weights)
+    ld_dout = _take_rows(dout, "dout", _F32, n, width, aligned=True)
+    n_experts = 0
     if offsets is not None:
-        d.n_experts, d.offsets = _take(offsets, "offsets", torch.int32, (None,)).shape[0] - 1, ptr(offsets)
-        if d.n_experts < 0:
+        n_experts = _take_vector(offsets, "offsets") - 1
+        if n_experts < 0:
             raise ValueError("offsets: [experts + 1] is wanted, got none")
-    d.dout, d.ld_dout = ptr(dout), _aligned_rows(dout, "dout")
-    _here(dout=dout, y=y, slot_of=slot_of, weights=weights, offsets=offsets)
-    dy, dweights = new(d.n_slots, d.width, y), new(d.n_rows, d.top_k, y)
-    d.dy, d.ld_dy, d.dweights = ptr(dy), d.width, ptr(dweights)
-    call("mb_experts_combine_bwd", C.byref(d), _stream())
+    device = _here(dout, y, slot_of, weights, offsets)
+    dy, dweights = torch.empty((n_slots, width), dtype=_F32, device=y.device), torch.empty((n, k), dtype=_F32, device=y.device)
+    _launch("mb_experts_combine_bwd", _lib.MbCombine, _COMBINE_FMT.pack(
+        n, n_slots, k, width, n_experts, 0, slot_of.data_ptr(), ptr(offsets) or 0, ptr(weights) or 0, y.data_ptr(), ld, 0, 0, dout.data_ptr(),
+        ld_dout, dy.data_ptr(), width, dweights.data_ptr()), device)
     return dy, dweights
 
 
