@@ -16,6 +16,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <initializer_list>
+#include <type_traits>
 #include "common.cuh"
 
 namespace mb {
@@ -154,64 +155,76 @@ __device__ __forceinline__ void join(float& na, float& ma, float& sa, float nb, 
 }
 
 // A block's shared memory: per-channel pairs of every warp or row lane, and the groups' results
-struct GnShared {
-  float first[GN_THREADS * 8], second[GN_THREADS * 8];  // [entries][width]
+template <int W> struct GnShared {
+  float first[GN_THREADS * W], second[GN_THREADS * W];  // [entries][width]
   float count[GN_THREADS];
   float group[2][GN_MAX_CHANNELS];
 };
 
-template <typename T, int V, int NC>
-__device__ __forceinline__ const Vec<T, V>* at(const void* base, int64_t row, int64_t ld, int c) {
-  return reinterpret_cast<const Vec<T, V>*>(static_cast<const T*>(base) + row * ld + c);
+// A thread's rows of [from, to), n of them, `step` bytes apart.  f(q, rows, whole) for its batches of U rows: `whole` is true_type where all
+// U are there, so that the bulk of the loop has no comparisons (with 64-bit row numbers compared and multiplied for every access a value
+// took 34 instructions in the forward pass, and the multiprocessors issued every other cycle at half the copy rate).
+template <int V> __device__ __forceinline__ int thread_rows(const Place<V>& p, int64_t from, int64_t to) {
+  return p.used && to - from > p.ty ? (int)((to - from - p.ty + p.ty_n - 1) / p.ty_n) : 0;
 }
+template <int U, typename F> __device__ __forceinline__ void batches(int n, F f) {
+  int left = n;
+  for (; left >= U; left -= U) f(U, std::true_type{});
+  if (left > 0) f(left, std::false_type{});
+}
+template <typename T, int V> struct Stream {
+  const char* p;
+  int64_t step;
+  __device__ __forceinline__ Stream(const void* base, int64_t ld, const Place<V>& at, int64_t from, int c)
+      : p(reinterpret_cast<const char*>(static_cast<const T*>(base) + (from + at.ty) * ld + c)), step((int64_t)sizeof(T) * ld * at.ty_n) {}
+  template <int U, typename W> __device__ __forceinline__ void read(Vec<T, V> (&v)[U], int rows, W) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (W::value || i < rows) v[i] = *reinterpret_cast<const Vec<T, V>*>(p);
+      p += step;
+    }
+  }
+  __device__ __forceinline__ void write(const Vec<T, V>& v) {
+    *reinterpret_cast<Vec<T, V>*>(const_cast<char*>(p)) = v;
+    p += step;
+  }
+};
 
 // means and squared deviations of [from, to) x [c0, c0 + width) into sh.group[0 / 1][group of the slab]
 template <typename T, int V, int NC>
-__device__ void block_stats(const GnArgs& a, GnShared& sh, int64_t from, int64_t to, int c0, int width, int cg) {
+__device__ void block_stats(const GnArgs& a, GnShared<V * NC>& sh, int64_t from, int64_t to, int c0, int width, int cg) {
   const Place<V> p(width);
-  float n = 0.f;
+  const int rows = thread_rows(p, from, to);
+  const float n_rows = (float)rows;
   Moments<V * NC> m;
   m.clear();
-  if (p.used) {
-    for (int64_t r0 = from + p.ty; r0 < to; r0 += (int64_t)GN_BATCH * p.ty_n) {
+  if (rows > 0) {
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        const int cv = p.tx + GN_THREADS * j;
-        if (NC > 1 && cv >= p.cols) break;
+    for (int j = 0; j < NC; ++j) {
+      const int cv = p.tx + GN_THREADS * j;
+      if (NC > 1 && cv >= p.cols) break;
+      Stream<T, V> x(a.x, a.ld_x, p, from, c0 + cv * V);
+      float n = 0.f;
+      batches<GN_BATCH>(rows, [&](int count, auto whole) {
         Vec<T, V> v[GN_BATCH];
-        float nb = 0.f;
-#pragma unroll
-        for (int i = 0; i < GN_BATCH; ++i) {
-          const int64_t r = r0 + (int64_t)i * p.ty_n;
-          if (r < to) { v[i] = *at<T, V, NC>(a.x, r, a.ld_x, c0 + cv * V); nb += 1.f; }
-          else v[i] = Vec<T, V>{};
-        }
-        const float inv = __fdividef(1.f, nb), f = __fdividef(nb, n + nb);
+        x.read(v, count, whole);
+        const float nb = (float)count, inv = __fdividef(1.f, nb), f = __fdividef(nb, n + nb);
         float sum[V], dev[V];
 #pragma unroll
         for (int c = 0; c < V; ++c) sum[c] = dev[c] = 0.f;
 #pragma unroll
         for (int i = 0; i < GN_BATCH; ++i) {
-          float x[V];
-          unpack(v[i], x);
-          add_to<V>(sum, x);
+          float t[V];
+          unpack(v[i], t);
+          if (decltype(whole)::value || i < count) add_to<V>(sum, t);
         }
 #pragma unroll
         for (int c = 0; c < V; ++c) sum[c] *= inv;
-        if (r0 + (int64_t)(GN_BATCH - 1) * p.ty_n < to) {
 #pragma unroll
-          for (int i = 0; i < GN_BATCH; ++i) {
-            float x[V];
-            unpack(v[i], x);
-            square_to<V>(dev, x, sum);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < GN_BATCH; ++i) {
-            float x[V];
-            unpack(v[i], x);
-            if (r0 + (int64_t)i * p.ty_n < to) square_to<V>(dev, x, sum);
-          }
+        for (int i = 0; i < GN_BATCH; ++i) {
+          float t[V];
+          unpack(v[i], t);
+          if (decltype(whole)::value || i < count) square_to<V>(dev, t, sum);
         }
 #pragma unroll
         for (int c = 0; c < V; ++c) {
@@ -220,10 +233,11 @@ __device__ void block_stats(const GnArgs& a, GnShared& sh, int64_t from, int64_t
           m.mean[k] = fmaf(d, f, m.mean[k]);
           m.m2[k] += dev[c] + d * d * n * f;
         }
-        if (j == NC - 1 || p.tx + GN_THREADS * (j + 1) >= p.cols) n += nb;
-      }
+        n += nb;
+      });
     }
   }
+  float n = n_rows;
   // lanes of a warp that hold the same channels, then warps (or row lanes) in shared memory
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool fold = p.tx_n < 32 && (p.tx_n & (p.tx_n - 1)) == 0;
@@ -310,23 +324,18 @@ __device__ __forceinline__ void load_stats(const float* stats, const Place<V>& p
 // y of [from, to) x [c0, c0 + width)
 template <typename T, int V, int NC, bool ACT>
 __device__ __forceinline__ void apply_rows(const GnArgs& a, const Place<V>& p, const Channels<V * NC>& k, int64_t from, int64_t to, int c0) {
-  if (!p.used) return;
-  T* const y = static_cast<T*>(a.y);
+  const int rows = thread_rows(p, from, to);
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
     const int cv = p.tx + GN_THREADS * j;
     if (NC > 1 && cv >= p.cols) break;
-    for (int64_t r0 = from + p.ty; r0 < to; r0 += (int64_t)GN_BATCH * p.ty_n) {
+    Stream<T, V> in(a.x, a.ld_x, p, from, c0 + cv * V), out(a.y, a.ld_y, p, from, c0 + cv * V);
+    batches<GN_BATCH>(rows, [&](int count, auto whole) {
       Vec<T, V> v[GN_BATCH];
+      in.read(v, count, whole);
 #pragma unroll
       for (int i = 0; i < GN_BATCH; ++i) {
-        const int64_t r = r0 + (int64_t)i * p.ty_n;
-        if (r < to) v[i] = *at<T, V, NC>(a.x, r, a.ld_x, c0 + cv * V);
-      }
-#pragma unroll
-      for (int i = 0; i < GN_BATCH; ++i) {
-        const int64_t r = r0 + (int64_t)i * p.ty_n;
-        if (r >= to) break;
+        if (!decltype(whole)::value && i >= count) break;
         float x[V];
         unpack(v[i], x);
         if constexpr (V == 1) {
@@ -342,9 +351,9 @@ __device__ __forceinline__ void apply_rows(const GnArgs& a, const Place<V>& p, c
         }
         Vec<T, V> o;
         pack(x, o);
-        *reinterpret_cast<Vec<T, V>*>(y + r * a.ld_y + c0 + cv * V) = o;
+        out.write(o);
       }
-    }
+    });
   }
 }
 template <typename T, int V, int NC>
@@ -382,7 +391,7 @@ __device__ __forceinline__ float rstd_of(float m2, float count, float eps) {
 template <typename T, int V, int NC, bool ACT>
 __global__ void __launch_bounds__(GN_THREADS, gn_blocks(V)) k_group_norm(const __grid_constant__ GnArgs a) {
   pdl_sync();
-  __shared__ GnShared sh;
+  __shared__ GnShared<V * NC> sh;
   const int cg = a.channels / a.groups, slabs = a.groups / a.slab_groups, width = cg * a.slab_groups;
   const int64_t units = (int64_t)a.n_seg * slabs;
   if (blockIdx.x >= units) {
@@ -426,10 +435,15 @@ __global__ void __launch_bounds__(GN_THREADS, gn_blocks(V)) k_group_norm(const _
 template <typename F> __device__ __forceinline__ void for_segments(const GnArgs& a, int64_t c_from, int64_t c_to, F f) {
   int64_t s = 0;
   if (a.seg_ptr) {  // the last segment that starts at or before c_from, or the first
-    int64_t lo = 0, hi = a.n_seg;
+    int64_t lo = 0, hi = a.n_seg;  // 32 probes at a time: two rounds for a thousand segments
     while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) / 2;
-      if ((int64_t)a.seg_ptr[mid] <= c_from) lo = mid; else hi = mid;
+      const int64_t step = (hi - lo + 31) / 32, at = lo + step * (threadIdx.x & 31);
+      const unsigned below = __ballot_sync(0xffffffffu, at < hi && (int64_t)a.seg_ptr[at] <= c_from);
+      // offsets are in order: the probes at or below c_from come first (whatever they hold, lo and hi close in)
+      const int n = __popc(below);
+      const int64_t next = n > 0 ? lo + step * (n - 1) : lo;
+      hi = min(next + step, hi);
+      lo = min(next, hi - 1);
     }
     s = lo;
   } else {
@@ -449,7 +463,7 @@ template <typename F> __device__ __forceinline__ void for_segments(const GnArgs&
 template <typename T, int V, int NC>
 __global__ void __launch_bounds__(GN_THREADS, gn_blocks(V)) k_group_norm_part(const __grid_constant__ GnArgs a) {
   pdl_sync();
-  __shared__ GnShared sh;
+  __shared__ GnShared<V * NC> sh;
   const int cg = a.channels / a.groups;
   const int64_t c_from = (int64_t)blockIdx.x * a.chunk, c_to = min(c_from + a.chunk, a.n_rows);
   for_segments(a, c_from, c_to, [&](int64_t s, int64_t from, int64_t to) {
@@ -512,27 +526,26 @@ __global__ void __launch_bounds__(GN_THREADS, gn_blocks(V)) k_group_norm_apply(c
 // ------------------------------------------------------------------ backward
 // Sums of dz and dz xh over [from, to), channel by channel, into sh.first[c], sh.second[c]
 template <typename T, int V, int NC, bool ACT>
-__device__ void block_sums(const GnArgs& a, GnShared& sh, const Place<V>& p, const Channels<V * NC>& k, int64_t from, int64_t to, int c0,
+__device__ void block_sums(const GnArgs& a, GnShared<V * NC>& sh, const Place<V>& p, const Channels<V * NC>& k, int64_t from, int64_t to, int c0,
                            int width) {
   float s1[V * NC], s2[V * NC];
 #pragma unroll
   for (int i = 0; i < V * NC; ++i) s1[i] = s2[i] = 0.f;
-  if (p.used) {
+  const int rows = thread_rows(p, from, to);
+  if (rows > 0) {
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
       const int cv = p.tx + GN_THREADS * j;
       if (NC > 1 && cv >= p.cols) break;
       constexpr int U = GN_BATCH / 2;
-      for (int64_t r0 = from + p.ty; r0 < to; r0 += (int64_t)U * p.ty_n) {
+      Stream<T, V> in(a.x, a.ld_x, p, from, c0 + cv * V), grad(a.dy, a.ld_dy, p, from, c0 + cv * V);
+      batches<U>(rows, [&](int count, auto whole) {
         Vec<T, V> v[U], d[U];
+        in.read(v, count, whole);
+        grad.read(d, count, whole);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-          const int64_t r = r0 + (int64_t)i * p.ty_n;
-          if (r < to) { v[i] = *at<T, V, NC>(a.x, r, a.ld_x, c0 + cv * V); d[i] = *at<T, V, NC>(a.dy, r, a.ld_dy, c0 + cv * V); }
-        }
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-          if (r0 + (int64_t)i * p.ty_n >= to) break;
+          if (!decltype(whole)::value && i >= count) break;
           float x[V], g[V];
           unpack(v[i], x);
           unpack(d[i], g);
@@ -552,7 +565,7 @@ __device__ void block_sums(const GnArgs& a, GnShared& sh, const Place<V>& p, con
             }
           }
         }
-      }
+      });
     }
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -592,24 +605,20 @@ __device__ void block_sums(const GnArgs& a, GnShared& sh, const Place<V>& p, con
 template <typename T, int V, int NC, bool ACT>
 __device__ __forceinline__ void gradient_rows(const GnArgs& a, const Place<V>& p, const Channels<V * NC>& k, const float (&m1)[V * NC],
                                               const float (&m2)[V * NC], int64_t from, int64_t to, int c0) {
-  if (!p.used) return;
-  T* const dx = static_cast<T*>(a.dx);
+  const int rows = thread_rows(p, from, to);
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
     const int cv = p.tx + GN_THREADS * j;
     if (NC > 1 && cv >= p.cols) break;
     constexpr int U = GN_BATCH / 2;
-    for (int64_t r0 = from + p.ty; r0 < to; r0 += (int64_t)U * p.ty_n) {
+    Stream<T, V> in(a.x, a.ld_x, p, from, c0 + cv * V), grad(a.dy, a.ld_dy, p, from, c0 + cv * V), out(a.dx, a.ld_dx, p, from, c0 + cv * V);
+    batches<U>(rows, [&](int count, auto whole) {
       Vec<T, V> v[U], d[U];
+      in.read(v, count, whole);
+      grad.read(d, count, whole);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        const int64_t r = r0 + (int64_t)i * p.ty_n;
-        if (r < to) { v[i] = *at<T, V, NC>(a.x, r, a.ld_x, c0 + cv * V); d[i] = *at<T, V, NC>(a.dy, r, a.ld_dy, c0 + cv * V); }
-      }
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int64_t r = r0 + (int64_t)i * p.ty_n;
-        if (r >= to) break;
+        if (!decltype(whole)::value && i >= count) break;
         float x[V], g[V];
         unpack(v[i], x);
         unpack(d[i], g);
@@ -629,14 +638,15 @@ __device__ __forceinline__ void gradient_rows(const GnArgs& a, const Place<V>& p
         }
         Vec<T, V> o;
         pack(x, o);
-        *reinterpret_cast<Vec<T, V>*>(dx + r * a.ld_dx + c0 + cv * V) = o;
+        out.write(o);
       }
-    }
+    });
   }
 }
 
 // the groups' means from a slab's channel sums: sh.group[0 / 1][group of the slab]
-__device__ __forceinline__ void group_means(const GnArgs& a, GnShared& sh, const float* first, const float* second, int stride, int c0, int width,
+template <int W>
+__device__ __forceinline__ void group_means(const GnArgs& a, GnShared<W>& sh, const float* first, const float* second, int stride, int c0, int width,
                                             int cg, float count) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int g = warp; g < width / cg; g += GN_WARPS) {
@@ -657,7 +667,7 @@ __device__ __forceinline__ void group_means(const GnArgs& a, GnShared& sh, const
   __syncthreads();
 }
 template <int V, int NC>
-__device__ __forceinline__ void load_means(const GnShared& sh, const Place<V>& p, int cg, float (&m1)[V * NC], float (&m2)[V * NC]) {
+__device__ __forceinline__ void load_means(const GnShared<V * NC>& sh, const Place<V>& p, int cg, float (&m1)[V * NC], float (&m2)[V * NC]) {
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
     const int cv = p.tx + GN_THREADS * j;
@@ -674,7 +684,7 @@ __device__ __forceinline__ void load_means(const GnShared& sh, const Place<V>& p
 template <typename T, int V, int NC, bool ACT>
 __global__ void __launch_bounds__(GN_THREADS, gn_blocks(V)) k_group_norm_bwd(const __grid_constant__ GnArgs a) {
   pdl_sync();
-  __shared__ GnShared sh;
+  __shared__ GnShared<V * NC> sh;
   const int cg = a.channels / a.groups, slabs = a.groups / a.slab_groups, width = cg * a.slab_groups;
   const int64_t units = (int64_t)a.n_seg * slabs;
   if (blockIdx.x >= units) {
@@ -705,7 +715,7 @@ __global__ void __launch_bounds__(GN_THREADS, gn_blocks(V)) k_group_norm_bwd(con
 template <typename T, int V, int NC, bool ACT>
 __global__ void __launch_bounds__(GN_THREADS, gn_blocks(V)) k_group_norm_bwd_part(const __grid_constant__ GnArgs a) {
   pdl_sync();
-  __shared__ GnShared sh;
+  __shared__ GnShared<V * NC> sh;
   const int cg = a.channels / a.groups;
   const int64_t c_from = (int64_t)blockIdx.x * a.chunk, c_to = min(c_from + a.chunk, a.n_rows);
   const Place<V> p(a.channels);
@@ -745,7 +755,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_group_norm_bwd_join(const __grid
 template <typename T, int V, int NC, bool ACT>
 __global__ void __launch_bounds__(GN_THREADS, gn_blocks(V)) k_group_norm_bwd_apply(const __grid_constant__ GnArgs a) {
   pdl_sync();
-  __shared__ GnShared sh;
+  __shared__ GnShared<V * NC> sh;
   const int64_t chunk = (int64_t)gridDim.x - 1 - blockIdx.x;
   const int64_t c_from = chunk * a.chunk, c_to = min(c_from + a.chunk, a.n_rows);
   const int cg = a.channels / a.groups;
@@ -802,11 +812,12 @@ static int gn_chunk(int64_t n_rows, int n_sm) {
   while (r < 512 && (int64_t)r * n_sm * 8 < n_rows) r *= 2;
   return r;
 }
-// Longest segment that one block takes per slab.  Streaming 128 bytes of a row at a time a block needs about 2 ns a row.
+// Longest segment that a block takes (slab by slab), -1: none.  Few rows: all of them, three launches fewer.  Segments that are long on
+// average: none.
 static int gn_limit(int64_t n_rows, int n_seg) {
-  constexpr int64_t most = 4096;
-  if (n_rows <= most / 4) return (int)most;
-  return n_rows > most * n_seg ? -1 : (int)most;
+  if (n_rows <= 1024) return 1024;
+  if (n_rows > 2048 * (int64_t)n_seg) return -1;
+  return n_rows <= 16384 ? 16384 : 4096;
 }
 static int gn_prepare(const mb_group_norm* d, GnArgs& a, int& n_sm) {
   int rc = sm_count(&n_sm);
@@ -826,11 +837,13 @@ static bool gn_vector(const mb_group_norm* d, std::initializer_list<const void*>
   for (int64_t ld : lds) if (ld % v) return false;
   return true;
 }
-// groups of a slab: as few as give 128 bytes of a row, whole vectors, slabs of one size
+// Groups of a slab: as few as give 128 bytes of a row and, segments being short, some 16 KB of a segment; whole vectors, slabs of one
+// size.  (256 segments of 36 rows of 512 bytes: 29 us by slabs of 64 bytes, 20 of 128, GN_SMALL_US whole.)
 static int gn_slab(const mb_group_norm* d, int v) {
-  const int size = d->dtype == MB_DTYPE_F32 ? 4 : 2, cg = d->channels / d->groups;
+  const int64_t size = d->dtype == MB_DTYPE_F32 ? 4 : 2, cg = d->channels / d->groups, average = d->n_rows / d->n_seg + 1;
+  const int64_t least = average < 128 ? 16384 / average : 128;
   for (int g = 1; g < d->groups; ++g)
-    if (d->groups % g == 0 && (g * cg) % v == 0 && g * cg * size >= 128 && g * cg / v <= GN_THREADS) return g;
+    if (d->groups % g == 0 && (g * cg) % v == 0 && g * cg * size >= least && g * cg / v <= GN_THREADS) return g;
   return d->groups;
 }
 template <typename F> static void gn_typed(int dtype, bool vec, F f) {
