@@ -23,7 +23,9 @@
 namespace mb {
 
 constexpr int GN_THREADS = 256, GN_WARPS = GN_THREADS / 32;
-constexpr int GN_BATCH = 8;            // rows of a thread in flight
+constexpr int GN_BATCH = 8;              // rows of a thread in flight, forward
+template <int V> constexpr int gn_pairs = V == 8 ? 2 : 4;  // ... and backward, of two tensors: eight 16-bit values a piece cost registers
+constexpr int GN_PLACES = 2;             // blocks of a multiprocessor that work by chunks
 constexpr int GN_MAX_CHANNELS = 1024;  // 256 threads, four channels each
 
 struct GnArgs {
@@ -504,12 +506,19 @@ __global__ void __launch_bounds__(GN_THREADS) k_group_norm_join(const __grid_con
   if (!by_chunks(a, to - from)) return;
   float n = 0.f, mean = 0.f, m2 = 0.f;
   if (from < to)
-    for (int64_t c = from / a.chunk + lane; c <= (to - 1) / a.chunk; c += 32) {
-      const int64_t f = max(from, c * a.chunk), t = min(to, (c + 1) * a.chunk);
-      const float* const part = a.part + 2 * ((c + s) * a.groups + g);
-      const float nb = (float)(t - f);
-      join(n, mean, m2, nb, part[0], part[1] / (float)cg);  // in units of rows: counts stay exact
-      n += nb;
+    for (int64_t c0 = from / a.chunk + lane; c0 <= (to - 1) / a.chunk; c0 += 32 * 8) {
+      float2 v[8];  // eight chunks' loads in flight
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + 32 * i <= (to - 1) / a.chunk) v[i] = *reinterpret_cast<const float2*>(a.part + 2 * ((c0 + 32 * i + s) * a.groups + g));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t c = c0 + 32 * i, f = max(from, c * a.chunk), t = min(to, (c + 1) * a.chunk);
+        if (f >= t) break;
+        const float nb = (float)(t - f);
+        join(n, mean, m2, nb, v[i].x, v[i].y / (float)cg);  // in units of rows: counts stay exact
+        n += nb;
+      }
     }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -555,7 +564,7 @@ __device__ void block_sums(const GnArgs& a, GnShared<V * NC>& sh, const Place<V>
     for (int j = 0; j < NC; ++j) {
       const int cv = p.tx + GN_THREADS * j;
       if (NC > 1 && cv >= p.cols) break;
-      constexpr int U = GN_BATCH / 2;
+      constexpr int U = gn_pairs<V>;
       Stream<T, V> in(a.x, a.ld_x, p, from, c0 + cv * V), grad(a.dy, a.ld_dy, p, from, c0 + cv * V);
       batches<U>(rows, [&](int count, auto whole) {
         Vec<T, V> v[U], d[U];
@@ -628,7 +637,7 @@ __device__ __forceinline__ void gradient_rows(const GnArgs& a, const Place<V>& p
   for (int j = 0; j < NC; ++j) {
     const int cv = p.tx + GN_THREADS * j;
     if (NC > 1 && cv >= p.cols) break;
-    constexpr int U = GN_BATCH / 2;
+    constexpr int U = gn_pairs<V>;
     Stream<T, V> in(a.x, a.ld_x, p, from, c0 + cv * V), grad(a.dy, a.ld_dy, p, from, c0 + cv * V), out(a.dx, a.ld_dx, p, from, c0 + cv * V);
     batches<U>(rows, [&](int count, auto whole) {
       Vec<T, V> v[U], d[U];
@@ -760,10 +769,14 @@ __global__ void __launch_bounds__(GN_THREADS) k_group_norm_bwd_join(const __grid
   if (!by_chunks(a, to - from)) return;
   float t1 = 0.f, t2 = 0.f;
   if (from < to)
-    for (int64_t ch = from / a.chunk + lane; ch <= (to - 1) / a.chunk; ch += 32) {
-      const float* const part = a.part + 2 * ((ch + s) * a.channels + c);
-      t1 += part[0];
-      t2 += part[1];
+    for (int64_t c0 = from / a.chunk + lane; c0 <= (to - 1) / a.chunk; c0 += 32 * 8) {
+      float2 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = c0 + 32 * i <= (to - 1) / a.chunk ? *reinterpret_cast<const float2*>(a.part + 2 * ((c0 + 32 * i + s) * a.channels + c))
+                                                 : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { t1 += v[i].x; t2 += v[i].y; }
     }
   t1 = warp_sum(t1);
   t2 = warp_sum(t2);
@@ -794,25 +807,34 @@ __global__ void __launch_bounds__(GN_THREADS, gn_blocks(V)) k_group_norm_bwd_app
   if (a.zero_rest) zero_rest<T, V, NC>(a, a.dx, a.ld_dx, (int)blockIdx.x, (int)gridDim.x);
 }
 
-// dw, db: a block takes 32 channels, its warps the segments in turn; 64-bit sums (a few KB, and segments may be many)
-__global__ void __launch_bounds__(GN_THREADS) k_group_norm_affine(const __grid_constant__ GnArgs a, float* __restrict__ dw,
-                                                                  float* __restrict__ db) {
+// dw, db: a block takes 32 channels, its 32 warps the segments in turn, eight loads in flight; 64-bit sums (a few KB, and segments may
+// be many)
+constexpr int GN_AFFINE_THREADS = 1024;
+__global__ void __launch_bounds__(GN_AFFINE_THREADS) k_group_norm_affine(const __grid_constant__ GnArgs a, float* __restrict__ dw,
+                                                                         float* __restrict__ db) {
   pdl_sync();
-  __shared__ double sh[GN_WARPS][2][32];
+  constexpr int WARPS = GN_AFFINE_THREADS / 32;
+  __shared__ double sh[WARPS][2][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane;
   double t1 = 0., t2 = 0.;
   if (c < a.channels)
-    for (int64_t s = warp; s < a.n_seg; s += GN_WARPS) {
-      const float2 v = *reinterpret_cast<const float2*>(a.sums + 2 * (s * a.channels + c));
-      t1 += (double)v.x;
-      t2 += (double)v.y;
+    for (int64_t s0 = warp; s0 < a.n_seg; s0 += 8 * WARPS) {
+      float2 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t s = s0 + i * WARPS;
+        v[i] = s < a.n_seg ? *reinterpret_cast<const float2*>(a.sums + 2 * (s * a.channels + c)) : make_float2(0.f, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { t1 += (double)v[i].x; t2 += (double)v[i].y; }
     }
   sh[warp][0][lane] = t1;
   sh[warp][1][lane] = t2;
   __syncthreads();
   if (warp < 2 && c < a.channels) {
     double t = 0.;
-    for (int i = 0; i < GN_WARPS; ++i) t += sh[i][warp][lane];
+#pragma unroll 8
+    for (int i = 0; i < WARPS; ++i) t += sh[i][warp][lane];
     float* const out = warp == 0 ? db : dw;
     if (out) out[c] = (float)t;
   }
@@ -825,10 +847,11 @@ static bool gn_valid(const mb_group_norm* d) {
   if (!d->seg_ptr && d->n_seg > 0 && d->n_rows % d->n_seg) return false;
   return d->n_rows <= INT32_MAX;
 }
+// Rows of a chunk: as many as put one block into each of GN_PLACES places of every multiprocessor, so that they all run at once.  (Every chunk
+// costs its block some 2 us beside the rows: 409,601 bf16 rows of 256 in chunks of 128 take 206 us, of 512 163, of 1,384 140.)
 static int gn_chunk(int64_t n_rows, int n_sm) {
-  int r = 32;
-  while (r < 512 && (int64_t)r * n_sm * 8 < n_rows) r *= 2;
-  return r;
+  const int64_t r = (n_rows + GN_PLACES * n_sm - 1) / (GN_PLACES * n_sm);
+  return (int)(r < 32 ? 32 : (r + 7) / 8 * 8);
 }
 // Longest segment that a block takes (slab by slab), -1: none.  Few rows: all of them, three launches fewer.  Segments that are long on
 // average: none.
@@ -856,7 +879,7 @@ static bool gn_vector(const mb_group_norm* d, std::initializer_list<const void*>
   return true;
 }
 // Groups of a slab: as few as give 128 bytes of a row and, segments being short, some 16 KB of a segment; whole vectors, slabs of one
-// size.  (256 segments of 36 rows of 512 bytes: 29 us by slabs of 64 bytes, 20 of 128, GN_SMALL_US whole.)
+// size.  (256 segments of 36 rows of 512 bytes: 29 us by slabs of 64 bytes, 20 of 128, 11 whole.)
 static int gn_slab(const mb_group_norm* d, int v) {
   const int64_t size = d->dtype == MB_DTYPE_F32 ? 4 : 2, cg = d->channels / d->groups, average = d->n_rows / d->n_seg + 1;
   const int64_t least = average < 128 ? 16384 / average : 128;
@@ -959,7 +982,7 @@ extern "C" int mb_group_norm_bwd(const mb_group_norm* d, void* stream) {
     a.n_seg = 0;
   }
   if (d->dweight || d->dbias) {
-    launch(k_group_norm_affine, (unsigned)cdiv(a.channels, 32), GN_THREADS, 0, st, a, d->dweight, d->dbias);
+    launch(k_group_norm_affine, (unsigned)cdiv(a.channels, 32), GN_AFFINE_THREADS, 0, st, a, d->dweight, d->dbias);
     MB_LAUNCH_CHECK("k_group_norm_affine");
   }
   return MB_OK;
