@@ -2,8 +2,9 @@
 // by expert, and the gradient; and the weighted sum that brings the experts' outputs back to their rows.
 //
 // A row is held by L neighbouring lanes, V experts each (L V >= n_experts), so that a warp works on 32 / L rows at once and a row's
-// reductions take log2 L shuffles.  Choices are made on 64-bit keys, the logit's order-preserving bits above the complement of its
-// index: the maximum of the keys is the largest logit and among equal ones the lowest index, in any order of comparison.
+// reductions take log2 L shuffles.  The selection is a chain of comparisons, and instructions bound it: with four experts a lane, 64-bit
+// keys and expf, 573,894 rows of 32 experts took 89 us of this launch alone, with eight, 32-bit keys and the hardware's power of two 61.
+// Choices are made on the logits' order-preserving bits; a lane keeps the first of its equal ones, lanes compare columns.
 //
 // Grouping without atomics whose order could matter: a block takes a run of rows and counts its choices per expert (k_route), the
 // counts are scanned expert by expert (k_route_scan), and every block then gives its pairs their slots in row order
@@ -89,34 +90,30 @@ template <int L> __device__ __forceinline__ float lanes_max(float v) {
   for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-template <int L> __device__ __forceinline__ unsigned long long lanes_max(unsigned long long v) {
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) {
-    const unsigned long long w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = w > v ? w : v;
-  }
-  return v;
-}
-
-// 0 for an expert that is not available; NaN above everything, -0 equal to 0
-__device__ __forceinline__ unsigned long long choice_key(float x, int column) {
-  if (x == MINUS_INF) return 0;
+// The logit's order as an unsigned number: 0 for an expert that is not available, NaN above everything, -0 equal to 0
+__device__ __forceinline__ uint32_t choice_key(float x) {
   uint32_t u = __float_as_uint(x + 0.f);
-  if (x != x) u = 0x7FC00000u;
   u = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-  return (unsigned long long)u << 32 | (0xFFFFFFFFu - (uint32_t)column);
+  if (x != x) u = 0xFFC00000u;
+  return x == MINUS_INF ? 0 : u;
 }
-__device__ __forceinline__ int key_column(unsigned long long k) { return (int)(0xFFFFFFFFu - (uint32_t)k); }
-__device__ __forceinline__ float key_value(unsigned long long k) {
-  const uint32_t u = (uint32_t)(k >> 32);
-  return __uint_as_float((u & 0x80000000u) ? u & 0x7FFFFFFFu : ~u);
+__device__ __forceinline__ float key_value(uint32_t u) { return __uint_as_float((u & 0x80000000u) ? u & 0x7FFFFFFFu : ~u); }
+// the larger key of a row's lanes, of equal ones the one of the lower column
+template <int L> __device__ __forceinline__ void lanes_best(uint32_t& key, int& column) {
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) {
+    const uint32_t k = __shfl_xor_sync(0xffffffffu, key, o);
+    const int c = __shfl_xor_sync(0xffffffffu, column, o);
+    if (k > key || (k == key && c < column)) { key = k; column = c; }
+  }
 }
+// exp(x), x <= 0: the hardware's power of two of x log2 e, off by some |x| 2^-24 (expf, exact to a step, took a third of a row's instructions)
+__device__ __forceinline__ float exp_below(float x) { return __expf(x); }
 
 // Rows [from, to) of a block: choices and weights to memory, choices counted in hist[], rows routed returned per thread, column sums
 // of the probabilities left in cols[0 .. n_experts)
-template <typename T, int L, int V, bool VEC>
+template <typename T, int L, int V, int Q, bool VEC>
 __device__ __forceinline__ void route_rows(const RtArgs& a, int64_t from, int64_t to, int32_t* hist, float (*cols)[L * V]) {
-  constexpr int Q = L >= 32 ? 1 : L == 16 ? 2 : 4;  // choices of a lane: top_k <= min(4 L, 32)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L, c0 = sub * V, n = a.n_experts, k = a.top_k;
   const T* const logits = static_cast<const T*>(a.logits);
   for (int i = threadIdx.x; i <= n; i += RT_THREADS) hist[i] = 0;
@@ -126,42 +123,52 @@ __device__ __forceinline__ void route_rows(const RtArgs& a, int64_t from, int64_
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
   int routed_rows = 0;
   constexpr int STEP = RT_THREADS / L;
+  // The next row is asked for before this one is worked on: a row's selection is a chain of shuffles that leaves the loads time enough.
+  float ahead[V];
+  auto ask = [&](int64_t t) {
+    const bool use = t < to && (!a.valid || a.valid[t]);
+    if (use) load_logits<T, V, VEC>(logits + t * a.ld, c0, n, ahead);
+    else
+#pragma unroll
+      for (int i = 0; i < V; ++i) ahead[i] = MINUS_INF;
+  };
+  ask(from + warp * (32 / L) + lane / L);
   for (int64_t t0 = from + warp * (32 / L); t0 < to; t0 += STEP) {  // the same for all lanes of a warp: shuffles need them
     const int64_t t = t0 + lane / L;
     const bool in = t < to;
     float x[V];
-    const bool use = in && (!a.valid || a.valid[t]);
-    if (use) load_logits<T, V, VEC>(logits + t * a.ld, c0, n, x);
-    else
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[i] = MINUS_INF;
-    unsigned long long key[V];
+    for (int i = 0; i < V; ++i) x[i] = ahead[i];
+    ask(t + STEP);
+    uint32_t key[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = choice_key(x[i], c0 + i);
-    int id[Q];
+    for (int i = 0; i < V; ++i) key[i] = choice_key(x[i]);
+    int id[Q];       // this lane's choices: every L-th, Q >= top_k / L
     float e_of[Q];
     float m = 0.f, total = 0.f, chosen = 0.f;
     bool routed = false;
     for (int j = 0; j < k; ++j) {
-      unsigned long long best = key[0];
+      uint32_t best = key[0];
+      int column = c0;
 #pragma unroll
-      for (int i = 1; i < V; ++i) best = key[i] > best ? key[i] : best;
-      best = lanes_max<L>(best);
+      for (int i = 1; i < V; ++i)
+        if (key[i] > best) { best = key[i]; column = c0 + i; }
+      lanes_best<L>(best, column);
       if (j == 0) {
         routed = best != 0;
         m = routed ? key_value(best) : 0.f;
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) { x[i] = x[i] == MINUS_INF ? 0.f : expf(x[i] - m); s += x[i]; }
+        for (int i = 0; i < V; ++i) { x[i] = x[i] == MINUS_INF ? 0.f : exp_below(x[i] - m); s += x[i]; }
         total = lanes_sum<L>(s);
       }
 #pragma unroll
-      for (int i = 0; i < V; ++i) key[i] = key[i] == best ? 0 : key[i];
-      const float e = best ? expf(key_value(best) - m) : 0.f;
+      for (int i = 0; i < V; ++i) key[i] = c0 + i == column ? 0 : key[i];
+      const float e = best ? exp_below(key_value(best) - m) : 0.f;
       chosen += e;
 #pragma unroll
       for (int q = 0; q < Q; ++q)
-        if (j == q * L + sub) { id[q] = best ? key_column(best) : -1; e_of[q] = e; }
+        if (j == q * L + sub) { id[q] = best ? column : -1; e_of[q] = e; }
     }
     if (in) {
       const float scale = routed ? 1.f / (a.renorm ? chosen : total) : 0.f;
@@ -193,12 +200,12 @@ __device__ __forceinline__ void route_rows(const RtArgs& a, int64_t from, int64_
   __syncthreads();
 }
 
-template <typename T, int L, int V, bool VEC> __global__ void __launch_bounds__(RT_THREADS) k_route(const __grid_constant__ RtArgs a) {
+template <typename T, int L, int V, int Q, bool VEC> __global__ void __launch_bounds__(RT_THREADS) k_route(const __grid_constant__ RtArgs a) {
   pdl_sync();
   __shared__ int32_t hist[RT_MAX_EXPERTS + 1];
   __shared__ float cols[RT_WARPS][L * V];
   const int64_t from = min((int64_t)blockIdx.x * a.block_rows, a.n_rows), to = min(from + a.block_rows, a.n_rows);
-  route_rows<T, L, V, VEC>(a, from, to, hist, cols);
+  route_rows<T, L, V, Q, VEC>(a, from, to, hist, cols);
   for (int e = threadIdx.x; e <= a.n_experts; e += RT_THREADS) {
     a.c_part[(int64_t)e * a.n_blocks + blockIdx.x] = hist[e];
     if (e < a.n_experts) {
@@ -217,20 +224,28 @@ __global__ void __launch_bounds__(RT_THREADS) k_route_scan(const __grid_constant
   if (e > a.n_experts) return;
   int32_t* const c = a.c_part + (int64_t)e * a.n_blocks;
   const float* const p = a.p_part + (int64_t)e * a.n_blocks;
-  int32_t before = 0;
+  // a lane takes a run of blocks: its sum, a scan over the lanes, then its exclusive sums
+  const int per = (a.n_blocks + 31) / 32, b0 = min(lane * per, a.n_blocks), b1 = min(b0 + per, a.n_blocks);
+  int32_t mine = 0;
   double sum = 0.;
-  for (int b0 = 0; b0 < a.n_blocks; b0 += 32) {
-    const int b = b0 + lane;
-    const int32_t v = b < a.n_blocks ? c[b] : 0;
-    if (e < a.n_experts && b < a.n_blocks) sum += (double)p[b];
-    int32_t s = v;
+#pragma unroll 8
+  for (int b = b0; b < b1; ++b) mine += c[b];
+  if (e < a.n_experts)
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) sum += (double)p[b];
+  int32_t upto = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
-    }
-    if (b < a.n_blocks) c[b] = before + s - v;
-    before += __shfl_sync(0xffffffffu, s, 31);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int32_t u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  const int32_t before = __shfl_sync(0xffffffffu, upto, 31);
+  int32_t at = upto - mine;
+#pragma unroll 8
+  for (int b = b0; b < b1; ++b) {
+    const int32_t v = c[b];
+    c[b] = at;
+    at += v;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -333,13 +348,13 @@ __global__ void __launch_bounds__(RT_THREADS) k_route_place(const __grid_constan
   place_pairs(a, from, min(from + a.block_rows, a.n_rows), base, of_warp);
 }
 
-template <typename T, int L, int V, bool VEC> __global__ void __launch_bounds__(RT_THREADS) k_route_small(const __grid_constant__ RtArgs a) {
+template <typename T, int L, int V, int Q, bool VEC> __global__ void __launch_bounds__(RT_THREADS) k_route_small(const __grid_constant__ RtArgs a) {
   pdl_sync();
   __shared__ int32_t hist[RT_MAX_EXPERTS + 1], base[RT_MAX_EXPERTS + 1];
   constexpr int COLS = RT_WARPS * L * V * 4, OF = RT_WARPS * RT_MAX_EXPERTS * 4;
   __shared__ __align__(16) uint8_t both[COLS > OF ? COLS : OF];
   float (*cols)[L * V] = reinterpret_cast<float (*)[L * V]>(both);
-  route_rows<T, L, V, VEC>(a, 0, a.n_rows, hist, cols);
+  route_rows<T, L, V, Q, VEC>(a, 0, a.n_rows, hist, cols);
   const int n = a.n_experts;
   for (int e = threadIdx.x; e <= n; e += RT_THREADS) a.counts[e] = hist[e];
   first_slots(hist, n, base);
@@ -360,9 +375,8 @@ template <typename T, int L, int V, bool VEC> __global__ void __launch_bounds__(
   place_pairs(a, 0, a.n_rows, base, reinterpret_cast<int32_t (*)[RT_MAX_EXPERTS]>(both));
 }
 
-template <typename T, int L, int V, bool VEC> __global__ void __launch_bounds__(RT_THREADS) k_route_bwd(const __grid_constant__ RtArgs a) {
+template <typename T, int L, int V, int Q, bool VEC> __global__ void __launch_bounds__(RT_THREADS) k_route_bwd(const __grid_constant__ RtArgs a) {
   pdl_sync();
-  constexpr int Q = L >= 32 ? 1 : L == 16 ? 2 : 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L, c0 = sub * V, n = a.n_experts, k = a.top_k;
   const T* const logits = static_cast<const T*>(a.logits);
   T* const dlogits = static_cast<T*>(a.dlogits);
@@ -371,34 +385,52 @@ template <typename T, int L, int V, bool VEC> __global__ void __launch_bounds__(
   const double unit = a.dloss && rows > 0 ? (double)*a.dloss * (double)n / ((double)k * (double)rows * (double)rows) : 0.;
 #pragma unroll
   for (int i = 0; i < V; ++i) share[i] = c0 + i < n ? (float)(unit * (double)a.counts[c0 + i]) : 0.f;
-  const int64_t step = (int64_t)gridDim.x * (RT_THREADS / L);
-  for (int64_t t0 = ((int64_t)blockIdx.x * RT_WARPS + warp) * (32 / L); t0 < a.n_rows; t0 += step) {
-    const int64_t t = t0 + lane / L;
+  const int64_t step = (int64_t)gridDim.x * (RT_THREADS / L), first = ((int64_t)blockIdx.x * RT_WARPS + warp) * (32 / L);
+  int next_id[Q];  // the next row's, asked for before this one is worked on
+  float next_dw[Q], next_w[Q], next_x[V];
+  auto ask = [&](int64_t t) {
     const bool in = t < a.n_rows;
-    int id[Q];
-    float dw[Q], w[Q];
-    float dot = 0.f;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int j = q * L + sub;
-      id[q] = in && j < k ? a.ids[t * k + j] : -1;
-      dw[q] = id[q] >= 0 && a.dweights ? a.dweights[t * k + j] : 0.f;
-      w[q] = id[q] >= 0 && a.renorm ? a.weights[t * k + j] : 0.f;
-      dot = id[q] >= 0 ? fmaf(w[q], dw[q], dot) : dot;
+      const bool use = in && j < k;
+      next_id[q] = use ? a.ids[t * k + j] : -1;
+      next_dw[q] = use && a.dweights ? a.dweights[t * k + j] : 0.f;
+      next_w[q] = use && a.renorm ? a.weights[t * k + j] : 0.f;
     }
-    const bool routed = __shfl_sync(0xffffffffu, id[0], lane - sub) >= 0;
-    float x[V];
-    if (routed) load_logits<T, V, VEC>(logits + t * a.ld, c0, n, x);
+    if (in) load_logits<T, V, VEC>(logits + t * a.ld, c0, n, next_x);
     else
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[i] = MINUS_INF;
+      for (int i = 0; i < V; ++i) next_x[i] = MINUS_INF;
+  };
+  ask(first + lane / L);
+  for (int64_t t0 = first; t0 < a.n_rows; t0 += step) {
+    const int64_t t = t0 + lane / L;
+    const bool in = t < a.n_rows;
+    int id[Q];
+    float dw[Q], w[Q], x[V];
+    float dot = 0.f;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) id[q] = next_id[q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) { dw[q] = next_dw[q]; w[q] = next_w[q]; }
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = next_x[i];
+    ask(t + step);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      if (id[q] < 0) dw[q] = w[q] = 0.f;
+      else dot = fmaf(w[q], dw[q], dot);
+    }
+    // what a row that is not routed holds goes no further: its gradient is zero
+    const bool routed = __shfl_sync(0xffffffffu, id[0], lane - sub) >= 0;
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < V; ++i) m = fmaxf(m, x[i]);
     m = lanes_max<L>(m);
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) { x[i] = x[i] == MINUS_INF ? 0.f : expf(x[i] - m); s += x[i]; }
+    for (int i = 0; i < V; ++i) { x[i] = x[i] == MINUS_INF ? 0.f : exp_below(x[i] - m); s += x[i]; }
     s = lanes_sum<L>(s);
     const float inv = routed ? 1.f / s : 0.f;
     if (a.renorm) dot = lanes_sum<L>(dot);
@@ -508,34 +540,38 @@ static bool route_vector(const mb_route* d, const void* rows, int64_t ld) {
   const uintptr_t bytes = d->dtype == MB_DTYPE_F32 ? 16 : 8;
   return d->n_experts % 4 == 0 && ld % 4 == 0 && reinterpret_cast<uintptr_t>(rows) % bytes == 0;
 }
-// f.run<T, L, V, VEC>(): lanes of a row by the number of experts
-template <typename T, bool VEC, typename F> static void route_lanes(int n, F& f) {
-  if (n <= 4) f.template run<T, 1, 4, VEC>();
-  else if (n <= 8) f.template run<T, 2, 4, VEC>();
-  else if (n <= 16) f.template run<T, 4, 4, VEC>();
-  else if (n <= 32) f.template run<T, 8, 4, VEC>();
-  else if (n <= 64) f.template run<T, 16, 4, VEC>();
-  else if (n <= 128) f.template run<T, 32, 4, VEC>();
-  else if (n <= 256) f.template run<T, 32, 8, VEC>();
-  else f.template run<T, 32, 32, VEC>();
+// f.run<T, L, V, Q, VEC>(): lanes of a row by the number of experts, choices of a lane by top_k
+template <typename T, int L, int V, bool VEC, typename F> static void route_choices(int k, F& f) {
+  constexpr int most = L >= 32 ? 1 : L == 16 ? 2 : L == 8 ? 4 : 8;  // top_k <= 32 and <= L V
+  if (k <= L) f.template run<T, L, V, 1, VEC>();
+  else f.template run<T, L, V, most, VEC>();
 }
-template <typename F> static void route_typed(int dtype, bool vec, int n, F f) {
-  if (dtype == MB_DTYPE_F32) { if (vec) route_lanes<float, true>(n, f); else route_lanes<float, false>(n, f); }
-  else if (dtype == MB_DTYPE_BF16) { if (vec) route_lanes<__nv_bfloat16, true>(n, f); else route_lanes<__nv_bfloat16, false>(n, f); }
-  else { if (vec) route_lanes<__half, true>(n, f); else route_lanes<__half, false>(n, f); }
+template <typename T, bool VEC, typename F> static void route_lanes(int n, int k, F& f) {
+  if (n <= 8) route_choices<T, 1, 8, VEC>(k, f);
+  else if (n <= 16) route_choices<T, 2, 8, VEC>(k, f);
+  else if (n <= 32) route_choices<T, 4, 8, VEC>(k, f);
+  else if (n <= 64) route_choices<T, 8, 8, VEC>(k, f);
+  else if (n <= 128) route_choices<T, 16, 8, VEC>(k, f);
+  else if (n <= 256) route_choices<T, 32, 8, VEC>(k, f);
+  else route_choices<T, 32, 32, VEC>(k, f);
+}
+template <typename F> static void route_typed(int dtype, bool vec, int n, int k, F f) {
+  if (dtype == MB_DTYPE_F32) { if (vec) route_lanes<float, true>(n, k, f); else route_lanes<float, false>(n, k, f); }
+  else if (dtype == MB_DTYPE_BF16) { if (vec) route_lanes<__nv_bfloat16, true>(n, k, f); else route_lanes<__nv_bfloat16, false>(n, k, f); }
+  else { if (vec) route_lanes<__half, true>(n, k, f); else route_lanes<__half, false>(n, k, f); }
 }
 struct RouteFwd {
   const RtArgs& a; cudaStream_t st; bool small;
-  template <typename T, int L, int V, bool VEC> void run() const {
-    if (small) launch(k_route_small<T, L, V, VEC>, 1, RT_THREADS, 0, st, a);
-    else launch(k_route<T, L, V, VEC>, (unsigned)a.n_blocks, RT_THREADS, 0, st, a);
+  template <typename T, int L, int V, int Q, bool VEC> void run() const {
+    if (small) launch(k_route_small<T, L, V, Q, VEC>, 1, RT_THREADS, 0, st, a);
+    else launch(k_route<T, L, V, Q, VEC>, (unsigned)a.n_blocks, RT_THREADS, 0, st, a);
   }
 };
 struct RouteBwd {
   const RtArgs& a; cudaStream_t st; int n_sm;
-  template <typename T, int L, int V, bool VEC> void run() const {
+  template <typename T, int L, int V, int Q, bool VEC> void run() const {
     const int64_t want = (a.n_rows + RT_THREADS / L - 1) / (RT_THREADS / L), most = 8 * (int64_t)n_sm;
-    launch(k_route_bwd<T, L, V, VEC>, (unsigned)(want < most ? want : most), RT_THREADS, 0, st, a);
+    launch(k_route_bwd<T, L, V, Q, VEC>, (unsigned)(want < most ? want : most), RT_THREADS, 0, st, a);
   }
 };
 
@@ -565,7 +601,7 @@ extern "C" int mb_route_fwd(const mb_route* d, void* stream) {
   a.p_total = static_cast<double*>(d->scratch);
   a.p_part = reinterpret_cast<float*>(a.p_total + d->n_experts);
   a.c_part = reinterpret_cast<int32_t*>(a.p_part + (size_t)d->n_experts * a.n_blocks);
-  route_typed(d->dtype, route_vector(d, d->logits, d->ld_logits), d->n_experts, RouteFwd{a, st, small});
+  route_typed(d->dtype, route_vector(d, d->logits, d->ld_logits), d->n_experts, d->top_k, RouteFwd{a, st, small});
   if (!small) {
     launch(k_route_scan, (unsigned)cdiv(d->n_experts + 1, RT_WARPS), RT_THREADS, 0, st, a);
     launch(k_route_place, (unsigned)a.n_blocks, RT_THREADS, 0, st, a);
@@ -583,7 +619,7 @@ extern "C" int mb_route_bwd(const mb_route* d, void* stream) {
   if (rc) return rc;
   const RtArgs a = route_args(d);
   const bool vec = route_vector(d, d->logits, d->ld_logits) && route_vector(d, d->dlogits, d->ld_dlogits);
-  route_typed(d->dtype, vec, d->n_experts, RouteBwd{a, (cudaStream_t)stream, n_sm});
+  route_typed(d->dtype, vec, d->n_experts, d->top_k, RouteBwd{a, (cudaStream_t)stream, n_sm});
   MB_LAUNCH_CHECK("k_route_bwd");
   return MB_OK;
 }
