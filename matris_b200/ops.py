@@ -804,8 +804,8 @@ def _combine_args(y, slot_of, weights):
     (n_slots, width), (n, k) = y.shape, slot_of.shape
     if width % 4 or not width:
         raise NotImplementedError(f"widths that are multiples of 4, got {width}")
-    if k < 1 or n * k >= 1 << 31 or n_slots >= 1 << 31:
-        raise NotImplementedError(f"1 choice a row or more, fewer than 2**31 in all, got {n} x {k}")
+    if not 1 <= k <= 32 or n * k >= 1 << 31 or n_slots >= 1 << 31:
+        raise NotImplementedError(f"1 to 32 choices a row, fewer than 2**31 in all, got {n} x {k}")
     ld = _take_rows(y, "y", _F32, aligned=True)
     if weights is not None:
         _take(weights, "weights", _F32, (n, k))
