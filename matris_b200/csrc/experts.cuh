@@ -42,15 +42,21 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-// The products of K steps [from, to) of a chunk (four of them): A in tensor memory at ta (hi | lo), weight or column tiles at wb (hi | lo)
-__device__ __forceinline__ void chunk_products(uint32_t d_tmem, uint32_t ta, uint32_t wb, int from, int to, bool fresh) {
+// The products of K steps [from, to) of a chunk (four of them): A in tensor memory at ta (hi | lo), weight or column tiles at wb (hi | lo).
+// The large ones, hi hi, and the corrections, lo hi + hi lo, 2^-11 of them, have accumulators of their own: the tensor cores cut every sum
+// to float32, towards zero, and a correction added to a large sum costs as much of it as another product.
+__device__ __forceinline__ void large_products(uint32_t d_tmem, uint32_t ta, uint32_t wb, int from, int to, bool fresh) {
+  const uint64_t dbh = umma_desc(wb);
+#pragma unroll
+  for (int kk = from; kk < to; ++kk) umma_tf32_ts(d_tmem, ta + 8 * kk, dbh + (uint64_t)(2 * kk), (!fresh || kk > 0) ? 1u : 0u);
+}
+__device__ __forceinline__ void small_products(uint32_t d_tmem, uint32_t ta, uint32_t wb, int from, int to, bool fresh) {
   const uint64_t dbh = umma_desc(wb), dbl = umma_desc(wb + TC_TILE_BYTES);
 #pragma unroll
   for (int kk = from; kk < to; ++kk) {
     const uint64_t adv = (uint64_t)(2 * kk);
     umma_tf32_ts(d_tmem, ta + 32 + 8 * kk, dbh + adv, (!fresh || kk > 0) ? 1u : 0u);
     umma_tf32_ts(d_tmem, ta + 8 * kk, dbl + adv, 1u);
-    umma_tf32_ts(d_tmem, ta + 8 * kk, dbh + adv, 1u);
   }
 }
 
@@ -124,7 +130,8 @@ constexpr int EX_STAGES = 2;                                     // patches of a
 constexpr int EX_W_SLOTS = 3;                                    // weight tiles (hi and lo) in flight
 constexpr int EX_PATCH_OFF = EX_W_SLOTS * 2 * TC_TILE_BYTES;
 constexpr int EX_BAR_OFF = EX_PATCH_OFF + EX_PROD_WARPS * EX_STAGES * 32 * 128;
-constexpr int EX_SMEM_BYTES = EX_BAR_OFF + 256;
+constexpr int EX_BIAS_OFF = EX_BAR_OFF + 256;                    // an epilogue warp's 64 values of the bias
+constexpr int EX_SMEM_BYTES = EX_BIAS_OFF + 8 * 256;
 static_assert(EX_SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
 
 // x = hi + lo, hi rounded to 11 significant bits by integer arithmetic (the conversion instruction runs at an eighth of the rate: two of
@@ -142,10 +149,10 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
     if (threadIdx.x == 0) atomicOr(&g_gemm_status, 2);
     return;
   }
-  // a_ready[4] (4 producer warps) a_done[4] | w_ready[3] w_done[3] | d_full[2] d_free[2] (8 epilogue warps) | retired
+  // a_ready[4] (4 producer warps) a_done[4] | w_ready[3] w_done[3] | d_full d_free (8 epilogue warps) | retired
   const uint32_t bar0 = smem_u32(bars);
-  const uint32_t a_ready = bar0, a_done = bar0 + 32, w_ready = bar0 + 64, w_done = bar0 + 96, d_full = bar0 + 128, d_free = bar0 + 144,
-                 retired = bar0 + 160;
+  const uint32_t a_ready = bar0, a_done = bar0 + 32, w_ready = bar0 + 64, w_done = bar0 + 96, d_full = bar0 + 128, d_free = bar0 + 136,
+                 retired = bar0 + 144;
   const uint32_t ring = smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nb = d.n_out / 128, nch = d.n_in / TC_BK;
@@ -156,7 +163,8 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
     if (lane == 0) {
       for (int b = 0; b < 4; ++b) { mbar_init(a_ready + 8 * b, 4); mbar_init(a_done + 8 * b, 1); }
       for (int b = 0; b < EX_W_SLOTS; ++b) { mbar_init(w_ready + 8 * b, 1); mbar_init(w_done + 8 * b, 1); }
-      for (int b = 0; b < 2; ++b) { mbar_init(d_full + 8 * b, 1); mbar_init(d_free + 8 * b, 8); }
+      mbar_init(d_full, 1);
+      mbar_init(d_free, 8);
       mbar_init(retired, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -188,38 +196,39 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
     bool alive = true;
     uint32_t g = 0, k = 0, slot = 0, phase = 0;  // A chunks and column blocks so far; weight slot and its use
     // The tensor cores' queue is a few instructions deep: issuing a chunk's twelve takes as long as they do, and then a wait that finds its
-    // barrier open still takes 110 - 140 cycles, three of them a chunk.  So the next chunk's barriers are tested ahead of the last
-    // three instructions, and waited for only where that fails (200 -> 165 us).
+    // barrier open still takes 110 - 140 cycles, three of them a chunk.  So the next chunk's barriers are tested between this one's
+    // instructions, and waited for only where that fails.
     bool open = false;
     for (int it = 0; it < n_items; ++it) {
       for (int j = 0; j < per_item; ++j, ++k) {
-        const uint32_t acc = k & 1, d_tmem = tmem_u + 128u * acc;
         for (int c = 0; c < nch; ++c) {
           const uint32_t ga = g + c, ab = ga & 3;
           if (!open) {
             if (j == 0 && alive) alive = mbar_wait(a_ready + 8 * ab, (ga >> 2) & 1);
             if (alive) alive = mbar_wait(w_ready + 8 * slot, phase & 1);
-            if (c == 0 && k >= 2 && alive) alive = mbar_wait(d_free + 8 * acc, ((k >> 1) - 1) & 1);
+            if (c == 0 && k >= 1 && alive) alive = mbar_wait(d_free, (k - 1) & 1);
             alive = __all_sync(0xffffffffu, alive);
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t ta = tmem_u + 256 + 64 * ab, wb = ring_u + slot * 2 * TC_TILE_BYTES;
-          if (elected) chunk_products(d_tmem, ta, wb, 0, 3, c == 0);
-          __syncwarp();
           const uint32_t slot1 = slot + 1 == EX_W_SLOTS ? 0 : slot + 1, phase1 = slot1 == 0 ? phase + 1 : phase;
-          const bool block_ends = c == nch - 1, item_ends = block_ends && j == per_item - 1;
-          const uint32_t k1 = k + 1, g1 = ga + 1;
-          bool ok = mbar_test(w_ready + 8 * slot1, phase1 & 1);
-          if (item_ends || (!block_ends && j == 0)) ok = mbar_test(a_ready + 8 * (g1 & 3), (g1 >> 2) & 1) && ok;
-          if (block_ends && k1 >= 2) ok = mbar_test(d_free + 8 * (k1 & 1), ((k1 >> 1) - 1) & 1) && ok;
-          open = __all_sync(0xffffffffu, ok);
+          const bool block_ends = c == nch - 1;
+          const uint32_t g1 = ga + 1;
+          if (elected) large_products(tmem_u, ta, wb, 0, 4, c == 0);
+          __syncwarp();
+          bool ok = !block_ends;  // the accumulators are never free this early
+          if (!block_ends && j == 0) ok = mbar_test(a_ready + 8 * (g1 & 3), (g1 >> 2) & 1);
+          if (elected) small_products(tmem_u + 128, ta, wb, 0, 3, c == 0);
+          __syncwarp();
+          ok = mbar_test(w_ready + 8 * slot1, phase1 & 1) && ok;
+          if (elected) small_products(tmem_u + 128, ta, wb, 3, 4, false);
+          __syncwarp();
           if (elected) {
-            chunk_products(d_tmem, ta, wb, 3, 4, false);
             if (j == per_item - 1) mma_commit(a_done + 8 * ab);
             mma_commit(w_done + 8 * slot);
-            if (block_ends) mma_commit(d_full + 8 * acc);
+            if (block_ends) mma_commit(d_full);
           }
-          __syncwarp();
+          open = __all_sync(0xffffffffu, ok);
           slot = slot1;
           phase = phase1;
         }
@@ -257,33 +266,38 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
     const int quarter = warp & 3, half = (warp - EX_EPI_WARP0) >> 2;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 64);
     const bool wide = ((reinterpret_cast<uintptr_t>(d.y) | reinterpret_cast<uintptr_t>(d.gate)) & 31u) == 0 && d.ld_y % 8 == 0 && d.ld_gate % 8 == 0;
+    float* const bias = reinterpret_cast<float*>(smem + EX_BIAS_OFF) + 64 * (warp - EX_EPI_WARP0);
+    *reinterpret_cast<float2*>(bias + 2 * lane) = make_float2(0.f, 0.f);
     bool alive = true;
     uint32_t k = 0;
     for (int item = blockIdx.x; walk.seek(item / per_tile, e, s0, rows); item += gridDim.x) {
       for (int jj = 0; jj < per_item; ++jj, ++k) {
-        const uint32_t acc = k & 1;
         const int c0 = 128 * (shared ? jj : item % nb) + 64 * half;
         const bool valid = quarter * 32 + lane < rows;
         const int64_t slot = s0 + (valid ? quarter * 32 + lane : 0);
         const float* const gate = d.gate ? d.gate + slot * d.ld_gate + c0 : nullptr;
-        const float* const bias = d.bias ? d.bias + (int64_t)e * d.n_out + c0 : nullptr;
         float* const out = d.y + slot * d.ld_y + c0;
+        // the products wait for the accumulators: no load from memory may stand between their reads
+        __syncwarp();
+        if (d.bias) *reinterpret_cast<float2*>(bias + 2 * lane) = *reinterpret_cast<const float2*>(d.bias + (int64_t)e * d.n_out + c0 + 2 * lane);
+        __syncwarp();
         if (gate) {
           asm volatile("prefetch.global.L2 [%0];" :: "l"(gate));
           asm volatile("prefetch.global.L2 [%0];" :: "l"(gate + 32));
         }
-        if (alive) alive = mbar_wait(d_full + 8 * acc, (k >> 1) & 1);
+        if (alive) alive = mbar_wait(d_full, k & 1);
         alive = __all_sync(0xffffffffu, alive);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
         for (int cg = 0; cg < 4; ++cg) {
-          uint32_t v[16];
-          MB_TMEM_LD16(lane_base + 128u * acc + 16u * cg, v);
+          uint32_t v[16], u[16];
+          MB_TMEM_LD16(lane_base + 16u * cg, v);
+          MB_TMEM_LD16(lane_base + 128u + 16u * cg, u);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
           if (cg == 3) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(d_free + 8 * acc);
+            if (lane == 0) mbar_arrive(d_free);
           }
           if (!alive || !valid) continue;
 #pragma unroll
@@ -291,12 +305,13 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
             const int c = cg * 16 + q * 8;
             float o[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(v[8 * q + i]);
-            if (bias) {
-              const float4 b0 = ld4(bias + c), b1 = ld4(bias + c + 4);
-              add4_to(o, b0);
-              add4_to(o + 4, b1);
-            }
+            for (int i = 0; i < 8; i += 2)
+              apart(two(__uint_as_float(v[8 * q + i]), __uint_as_float(v[8 * q + i + 1])) +
+                        two(__uint_as_float(u[8 * q + i]), __uint_as_float(u[8 * q + i + 1])),
+                    o[i], o[i + 1]);
+            const float4 b0 = ld4(bias + c), b1 = ld4(bias + c + 4);
+            add4_to(o, b0);
+            add4_to(o + 4, b1);
             if (gate) {
               const float4 z0 = ld4(gate + c), z1 = ld4(gate + c + 4);
               silu_grad4_to(o, z0);
