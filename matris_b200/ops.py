@@ -66,11 +66,13 @@ def as_split(W) -> SplitWeight:
         return W
     # an entry keeps W, so that its address is not handed out again; views of one storage differ in shape or strides
     key = (W.data_ptr(), tuple(W.shape), W.stride(), W._version)
-    entry = _split_cache.get(key)
+    entry = _split_cache.pop(key, None)
     if entry is None:
+        # the one used longest ago goes: never one that the call in progress has just looked up
         if len(_split_cache) > 256:
-            _split_cache.clear()
-        entry = _split_cache[key] = (W.detach(), SplitWeight(W))
+            del _split_cache[next(iter(_split_cache))]
+        entry = (W.detach(), SplitWeight(W))
+    _split_cache[key] = entry
     return entry[1]
 
 
@@ -573,7 +575,7 @@ def group_norm_fwd(x, weight, bias, n_groups, seg_ptr=None, eps=1e-5, act=0, out
     """Group norm with an optional SiLU (``act=1``), features last: every segment of rows and group of neighbouring channels
     has its own mean and variance (float32 arithmetic; x float32, bfloat16 or float16; weight and bias float32 [channels] or None).
 
-    ``x`` [rows, channels] with ``seg_ptr`` (int32 [segments + 1] row offsets on the device, as a batch's ``atom_ptr``), or
+    ``x`` [rows, channels] with ``seg_ptr`` (int32 [segments + 1] row offsets on the device, as ``BatchedGraph.atom_ptr``), or
     [batch, .., channels] without.  Returns (y, stats): stats [segments, groups, 2] (mean, 1 / deviation) is what
     ``group_norm_bwd`` reads.  Rows of no segment are zero in a returned tensor and left alone in a given ``out``, which may be x."""
     xr, rows, channels, ld, n_seg = _norm_rows(x, weight, bias, seg_ptr, n_groups, act, eps)
@@ -687,8 +689,11 @@ def route_bwd(logits, route: Route, dweights=None, dloss=None):
     _take(route.totals, "route.totals", _I32, (n_experts + 1,))
     if dweights is not None:
         _take(dweights, "dweights", _F32, shape)
-    if dloss is not None and (dloss.dtype != _F32 or dloss.numel() != 1):
-        raise ValueError(f"dloss: a float32 scalar is wanted, got {dloss.dtype}, shape {tuple(dloss.shape)}")
+    if dloss is not None:
+        if not isinstance(dloss, torch.Tensor) or dloss.dtype != _F32:
+            raise TypeError(f"dloss: a float32 tensor is wanted, got {getattr(dloss, 'dtype', type(dloss).__name__)}")
+        if dloss.numel() != 1:
+            raise ValueError(f"dloss: a scalar is wanted, got shape {tuple(dloss.shape)}")
     device = _here(logits, ids, route.weights, route.totals, dweights, dloss)
     dlogits = torch.empty((n, n_experts), dtype=logits.dtype, device=logits.device)
     _launch("mb_route_bwd", _lib.MbRoute, _ROUTE_FMT.pack(

@@ -19,3 +19,22 @@ def test_an_address_handed_out_again_is_not_taken_for_the_old_weight():
         w = torch.randn(128, 256)[:, :128]
         assert torch.equal(ops.as_split(w).w, w), i
         del w
+
+
+def test_a_full_cache_keeps_what_a_call_has_just_looked_up():
+    """A call looks up several weights and hands their addresses on together: making room for one must not free another, whether it
+    was new or had been there longest."""
+    ops._split_cache.clear()
+    weights = [torch.full((2, 4), float(i)) for i in range(400)]
+    try:
+        oldest = ops.as_split(weights[0])
+        for i in range(1, 300):
+            ops.as_split(weights[i])
+            assert ops.as_split(weights[0]) is oldest  # used all along
+            new, again = ops.as_split(weights[i]), ops.as_split(weights[0])
+            ops.as_split(weights[(i + 1) % 400])
+            kept = [e[1] for e in ops._split_cache.values()]
+            assert any(s is new for s in kept) and any(s is again for s in kept)
+        assert len(ops._split_cache) <= 258
+    finally:
+        ops._split_cache.clear()
