@@ -23,7 +23,13 @@ __device__ __forceinline__ const float* source_row(const mb_experts& d, int64_t 
 //
 // Operands are split into two tf32 parts, hi rounded to nearest: x = hi + lo to 2^-22, and the three products kept drop lo lo, at
 // most 2^-24 of |x w| and of either sign: the float32 rounding of the sums is as large.  (Two bf16 parts, as the other dense
-// layers have, are twice as fast and good to 2^-17: of no use here, where memory bounds the call either way.)
+// layers have, issue at twice the rate and are good to 2^-17.)
+//
+// 573,894 slots of 286,947 rows, 32 experts: 256 -> 128 in 217 us (174 TFLOP/s), 128 -> 256 in 258 (146).  Neither memory (90 and 135 us)
+// nor the tensor cores (115 us at their tf32 rate) set that: an instruction takes the warp that issues it some 50 cycles, twelve a chunk,
+// and a column block's accumulators are read out before the next block may use them.  One accumulator for both kinds of products, two of
+// them in turn, took 180 and 186 us and lost 1.1e-6 / 1.8e-6 of the result's norm with 128 / 256 terms where this loses 4e-7 / 9e-7; two
+// issuing warps, one for each kind, or sixteen epilogue warps 231 - 281 us.
 //
 // shared (K = 128): the four A buffers hold the whole row tile, converted once for all its column blocks.  Otherwise a column block is a
 // tile of its own and its rows are gathered again, from L2.
@@ -124,7 +130,7 @@ template <int SHIFT> struct Walk {
 };
 
 // A producer warp spends some 2,500 cycles on a chunk of 32 x 32 values, most of them waiting for its own instructions, where the chunk's
-// products take 768: sixteen of them, each chunk of four to a set of its own (eight, of two: 200 us where this takes 150).
+// products take 768: sixteen of them, each chunk of four to a set of its own.
 constexpr int EX_SETS = 4, EX_PROD_WARPS = 4 * EX_SETS, EX_EPI_WARP0 = PS_PROD_WARP0 + EX_PROD_WARPS, EX_THREADS = 32 * (EX_EPI_WARP0 + 8);
 constexpr int EX_STAGES = 2;                                     // patches of a producer warp
 constexpr int EX_W_SLOTS = 3;                                    // weight tiles (hi and lo) in flight
@@ -188,9 +194,8 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
     uint32_t elected;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0), ring_u = __shfl_sync(0xffffffffu, ring, 0);
-    // The number of this CTA's items, from one lane: the loop, and with it every operand of a matrix instruction, is then the same for all
-    // lanes by construction.  Where the compiler cannot see that it moves each operand to a uniform register in front of each instruction
-    // (walking the tiles here took 1,440 cycles a chunk for 768 of products).
+    // the number of this CTA's items, from one lane: the loop, and with it every operand of a matrix instruction, is the same for all lanes
+    // by construction
     const int64_t items = walk.count() * per_tile;
     const int n_items = __shfl_sync(0xffffffffu, (int)((items - blockIdx.x + gridDim.x - 1) / gridDim.x), 0);
     bool alive = true;
@@ -450,6 +455,9 @@ __global__ void __launch_bounds__(256) k_experts_split(int n_out, int n_in, int6
 // The tensor cores cut each sum they accumulate to float32 instead of rounding it, always towards zero: after n of them a sum is
 // short by up to n 2^-23.  So a run is accumulated there for EG_FLUSH chunks only and added up in float32 registers of the epilogue
 // warps, rounded to nearest.
+//
+// 573,894 slots, 256 -> 128, 32 experts: 297 us (127 TFLOP/s).  The column warps bound it, some 2,000 cycles a chunk of their own
+// instructions where its products take 768; sixteen of them do not fit the registers beside the epilogue's sums.
 //
 // Roles: warp 0 issues the products, warps 2 - 5 hold dy's columns, 6 - 9 x's, 10 - 17 the sums (warp 1 has none).
 constexpr int EG_FLUSH = 4;

@@ -65,6 +65,7 @@ PTR = torch.tensor([0, 4], dtype=I)
     (ValueError, lambda: ops.experts_grad_w(x(4, 128), x(0, 128), PTR, idx=torch.zeros(4, dtype=I))),
     (NotImplementedError, lambda: ops.experts_combine_fwd(x(4, 6), torch.zeros(2, 2, dtype=I))),
     (NotImplementedError, lambda: ops.experts_combine_fwd(x(4, 8), torch.zeros(2, 0, dtype=I))),
+    (NotImplementedError, lambda: ops.experts_combine_fwd(x(4, 8), torch.zeros(2, 33, dtype=I))),
     (ValueError, lambda: ops.experts_combine_fwd(x(4, 8), torch.zeros(2, 2, dtype=I), x(2, 3))),
     (TypeError, lambda: ops.experts_combine_fwd(x(4, 8), torch.zeros(2, 2))),
     (ValueError, lambda: ops.experts_combine_bwd(x(2, 9), x(4, 8), torch.zeros(2, 2, dtype=I))),
