@@ -132,6 +132,9 @@ template <int SHIFT> struct Walk {
 // A producer warp spends some 2,500 cycles on a chunk of 32 x 32 values, most of them waiting for its own instructions, where the chunk's
 // products take 768: sixteen of them, each chunk of four to a set of its own.
 constexpr int EX_SETS = 4, EX_PROD_WARPS = 4 * EX_SETS, EX_EPI_WARP0 = PS_PROD_WARP0 + EX_PROD_WARPS, EX_THREADS = 32 * (EX_EPI_WARP0 + 8);
+// Chunks whose products go into the accumulators before these are read: with more than 256 values of K a row's sum is joined from such runs
+// in the epilogue, rounded to nearest, by way of the output (512 values in one run lost 1.4e-6 of the result's norm).
+constexpr int EX_RUN = 8;
 constexpr int EX_STAGES = 2;                                     // patches of a producer warp
 constexpr int EX_W_SLOTS = 3;                                    // weight tiles (hi and lo) in flight
 constexpr int EX_PATCH_OFF = EX_W_SLOTS * 2 * TC_TILE_BYTES;
@@ -199,31 +202,31 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
     const int64_t items = walk.count() * per_tile;
     const int n_items = __shfl_sync(0xffffffffu, (int)((items - blockIdx.x + gridDim.x - 1) / gridDim.x), 0);
     bool alive = true;
-    uint32_t g = 0, k = 0, slot = 0, phase = 0;  // A chunks and column blocks so far; weight slot and its use
+    uint32_t g = 0, run = 0, slot = 0, phase = 0;  // A chunks and uses of the accumulators so far; weight slot and its use
     // The tensor cores' queue is a few instructions deep: issuing a chunk's twelve takes as long as they do, and then a wait that finds its
     // barrier open still takes 110 - 140 cycles, three of them a chunk.  So the next chunk's barriers are tested between this one's
     // instructions, and waited for only where that fails.
     bool open = false;
     for (int it = 0; it < n_items; ++it) {
-      for (int j = 0; j < per_item; ++j, ++k) {
+      for (int j = 0; j < per_item; ++j) {
         for (int c = 0; c < nch; ++c) {
           const uint32_t ga = g + c, ab = ga & 3;
           if (!open) {
             if (j == 0 && alive) alive = mbar_wait(a_ready + 8 * ab, (ga >> 2) & 1);
             if (alive) alive = mbar_wait(w_ready + 8 * slot, phase & 1);
-            if (c == 0 && k >= 1 && alive) alive = mbar_wait(d_free, (k - 1) & 1);
+            if (c % EX_RUN == 0 && run >= 1 && alive) alive = mbar_wait(d_free, (run - 1) & 1);
             alive = __all_sync(0xffffffffu, alive);
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t ta = tmem_u + 256 + 64 * ab, wb = ring_u + slot * 2 * TC_TILE_BYTES;
           const uint32_t slot1 = slot + 1 == EX_W_SLOTS ? 0 : slot + 1, phase1 = slot1 == 0 ? phase + 1 : phase;
-          const bool block_ends = c == nch - 1;
+          const bool run_ends = c == nch - 1 || c % EX_RUN == EX_RUN - 1;
           const uint32_t g1 = ga + 1;
-          if (elected) large_products(tmem_u, ta, wb, 0, 4, c == 0);
+          if (elected) large_products(tmem_u, ta, wb, 0, 4, c % EX_RUN == 0);
           __syncwarp();
-          bool ok = !block_ends;  // the accumulators are never free this early
-          if (!block_ends && j == 0) ok = mbar_test(a_ready + 8 * (g1 & 3), (g1 >> 2) & 1);
-          if (elected) small_products(tmem_u + 128, ta, wb, 0, 3, c == 0);
+          bool ok = !run_ends;  // the accumulators are never free this early
+          if (!run_ends && j == 0) ok = mbar_test(a_ready + 8 * (g1 & 3), (g1 >> 2) & 1);
+          if (elected) small_products(tmem_u + 128, ta, wb, 0, 3, c % EX_RUN == 0);
           __syncwarp();
           ok = mbar_test(w_ready + 8 * slot1, phase1 & 1) && ok;
           if (elected) small_products(tmem_u + 128, ta, wb, 3, 4, false);
@@ -231,8 +234,9 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
           if (elected) {
             if (j == per_item - 1) mma_commit(a_done + 8 * ab);
             mma_commit(w_done + 8 * slot);
-            if (block_ends) mma_commit(d_full);
+            if (run_ends) mma_commit(d_full);
           }
+          if (run_ends) ++run;
           open = __all_sync(0xffffffffu, ok);
           slot = slot1;
           phase = phase1;
@@ -274,9 +278,9 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
     float* const bias = reinterpret_cast<float*>(smem + EX_BIAS_OFF) + 64 * (warp - EX_EPI_WARP0);
     *reinterpret_cast<float2*>(bias + 2 * lane) = make_float2(0.f, 0.f);
     bool alive = true;
-    uint32_t k = 0;
+    uint32_t run = 0;
     for (int item = blockIdx.x; walk.seek(item / per_tile, e, s0, rows); item += gridDim.x) {
-      for (int jj = 0; jj < per_item; ++jj, ++k) {
+      for (int jj = 0; jj < per_item; ++jj) {
         const int c0 = 128 * (shared ? jj : item % nb) + 64 * half;
         const bool valid = quarter * 32 + lane < rows;
         const int64_t slot = s0 + (valid ? quarter * 32 + lane : 0);
@@ -290,41 +294,48 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
           asm volatile("prefetch.global.L2 [%0];" :: "l"(gate));
           asm volatile("prefetch.global.L2 [%0];" :: "l"(gate + 32));
         }
-        if (alive) alive = mbar_wait(d_full, k & 1);
-        alive = __all_sync(0xffffffffu, alive);
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (int c_run = 0; c_run < nch; c_run += EX_RUN, ++run) {
+          const bool first = c_run == 0, last = c_run + EX_RUN >= nch;
+          if (alive) alive = mbar_wait(d_full, run & 1);
+          alive = __all_sync(0xffffffffu, alive);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-        for (int cg = 0; cg < 4; ++cg) {
-          uint32_t v[16], u[16];
-          MB_TMEM_LD16(lane_base + 16u * cg, v);
-          MB_TMEM_LD16(lane_base + 128u + 16u * cg, u);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          if (cg == 3) {
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(d_free);
-          }
-          if (!alive || !valid) continue;
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int c = cg * 16 + q * 8;
-            float o[8];
-#pragma unroll
-            for (int i = 0; i < 8; i += 2)
-              apart(two(__uint_as_float(v[8 * q + i]), __uint_as_float(v[8 * q + i + 1])) +
-                        two(__uint_as_float(u[8 * q + i]), __uint_as_float(u[8 * q + i + 1])),
-                    o[i], o[i + 1]);
-            const float4 b0 = ld4(bias + c), b1 = ld4(bias + c + 4);
-            add4_to(o, b0);
-            add4_to(o + 4, b1);
-            if (gate) {
-              const float4 z0 = ld4(gate + c), z1 = ld4(gate + c + 4);
-              silu_grad4_to(o, z0);
-              silu_grad4_to(o + 4, z1);
+          for (int cg = 0; cg < 4; ++cg) {
+            uint32_t v[16], u[16];
+            MB_TMEM_LD16(lane_base + 16u * cg, v);
+            MB_TMEM_LD16(lane_base + 128u + 16u * cg, u);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (cg == 3) {
+              asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) mbar_arrive(d_free);
             }
-            if (d.out_act) silu_fast_all(o, o);
-            if (wide) st8(out + c, o);
-            else { st4(out + c, make_float4(o[0], o[1], o[2], o[3])); st4(out + c + 4, make_float4(o[4], o[5], o[6], o[7])); }
+            if (!alive || !valid) continue;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int c = cg * 16 + q * 8;
+              float o[8];
+#pragma unroll
+              for (int i = 0; i < 8; i += 2)
+                apart(two(__uint_as_float(v[8 * q + i]), __uint_as_float(v[8 * q + i + 1])) +
+                          two(__uint_as_float(u[8 * q + i]), __uint_as_float(u[8 * q + i + 1])),
+                      o[i], o[i + 1]);
+              if (!first) {  // what this thread left there
+                add4_to(o, ld4(out + c));
+                add4_to(o + 4, ld4(out + c + 4));
+              }
+              if (last) {
+                add4_to(o, ld4(bias + c));
+                add4_to(o + 4, ld4(bias + c + 4));
+                if (gate) {
+                  silu_grad4_to(o, ld4(gate + c));
+                  silu_grad4_to(o + 4, ld4(gate + c + 4));
+                }
+                if (d.out_act) silu_fast_all(o, o);
+              }
+              if (wide) st8(out + c, o);
+              else { st4(out + c, make_float4(o[0], o[1], o[2], o[3])); st4(out + c + 4, make_float4(o[4], o[5], o[6], o[7])); }
+            }
           }
         }
       }
