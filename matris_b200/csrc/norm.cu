@@ -493,44 +493,44 @@ __global__ void __launch_bounds__(GN_THREADS, gn_blocks(V)) k_group_norm_part(co
   });
 }
 
-// warp per (segment, group): the chunks' statistics, each lane its chunks in order, then the lanes
+// Warp per (segment, group): the chunks' statistics, each lane its chunks in order, then the lanes.  blockIdx.x = segment, the blocks of
+// a segment take its groups in turn: most segments go by blocks, and theirs are gone after one look.
 __global__ void __launch_bounds__(GN_THREADS) k_group_norm_join(const __grid_constant__ GnArgs a) {
   pdl_sync();
-  const int64_t unit = (int64_t)blockIdx.x * GN_WARPS + (threadIdx.x >> 5);
+  const int64_t s = blockIdx.x;
   const int lane = threadIdx.x & 31, cg = a.channels / a.groups;
-  if (unit >= (int64_t)a.n_seg * a.groups) return;
-  const int64_t s = unit / a.groups;
-  const int g = (int)(unit % a.groups);
   int64_t from, to;
   segment_rows(a, s, from, to);
   if (!by_chunks(a, to - from)) return;
-  float n = 0.f, mean = 0.f, m2 = 0.f;
-  if (from < to)
-    for (int64_t c0 = from / a.chunk + lane; c0 <= (to - 1) / a.chunk; c0 += 32 * 8) {
-      float2 v[8];  // eight chunks' loads in flight
+  for (int g = blockIdx.y * GN_WARPS + (threadIdx.x >> 5); g < a.groups; g += gridDim.y * GN_WARPS) {
+    float n = 0.f, mean = 0.f, m2 = 0.f;
+    if (from < to)
+      for (int64_t c0 = from / a.chunk + lane; c0 <= (to - 1) / a.chunk; c0 += 32 * 8) {
+        float2 v[8];  // eight chunks' loads in flight
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c0 + 32 * i <= (to - 1) / a.chunk) v[i] = *reinterpret_cast<const float2*>(a.part + 2 * ((c0 + 32 * i + s) * a.groups + g));
+        for (int i = 0; i < 8; ++i)
+          if (c0 + 32 * i <= (to - 1) / a.chunk) v[i] = *reinterpret_cast<const float2*>(a.part + 2 * ((c0 + 32 * i + s) * a.groups + g));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t c = c0 + 32 * i, f = max(from, c * a.chunk), t = min(to, (c + 1) * a.chunk);
-        if (f >= t) break;
-        const float nb = (float)(t - f);
-        join(n, mean, m2, nb, v[i].x, v[i].y / (float)cg);  // in units of rows: counts stay exact
-        n += nb;
+        for (int i = 0; i < 8; ++i) {
+          const int64_t c = c0 + 32 * i, f = max(from, c * a.chunk), t = min(to, (c + 1) * a.chunk);
+          if (f >= t) break;
+          const float nb = (float)(t - f);
+          join(n, mean, m2, nb, v[i].x, v[i].y / (float)cg);  // in units of rows: counts stay exact
+          n += nb;
+        }
       }
-    }
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const float nb = __shfl_xor_sync(0xffffffffu, n, o), mo = __shfl_xor_sync(0xffffffffu, mean, o), so = __shfl_xor_sync(0xffffffffu, m2, o);
-    const bool low_lane = (lane & o) == 0;
-    float n1 = low_lane ? n : nb, m1 = low_lane ? mean : mo, s1 = low_lane ? m2 : so;
-    join(n1, m1, s1, low_lane ? nb : n, low_lane ? mo : mean, low_lane ? so : m2);
-    n += nb; mean = m1; m2 = s1;
-  }
-  if (lane == 0) {
-    a.stats[2 * unit] = mean;
-    a.stats[2 * unit + 1] = rstd_of(m2, n, a.eps);
+    for (int o = 1; o < 32; o <<= 1) {
+      const float nb = __shfl_xor_sync(0xffffffffu, n, o), mo = __shfl_xor_sync(0xffffffffu, mean, o), so = __shfl_xor_sync(0xffffffffu, m2, o);
+      const bool low_lane = (lane & o) == 0;
+      float n1 = low_lane ? n : nb, m1 = low_lane ? mean : mo, s1 = low_lane ? m2 : so;
+      join(n1, m1, s1, low_lane ? nb : n, low_lane ? mo : mean, low_lane ? so : m2);
+      n += nb; mean = m1; m2 = s1;
+    }
+    if (lane == 0) {
+      a.stats[2 * (s * a.groups + g)] = mean;
+      a.stats[2 * (s * a.groups + g) + 1] = rstd_of(m2, n, a.eps);
+    }
   }
 }
 
@@ -756,31 +756,30 @@ __global__ void __launch_bounds__(GN_THREADS, gn_blocks(V)) k_group_norm_bwd_par
   });
 }
 
-// warp per (segment, channel): the chunks' sums
+// the same for the channels' sums
 __global__ void __launch_bounds__(GN_THREADS) k_group_norm_bwd_join(const __grid_constant__ GnArgs a) {
   pdl_sync();
-  const int64_t unit = (int64_t)blockIdx.x * GN_WARPS + (threadIdx.x >> 5);
+  const int64_t s = blockIdx.x;
   const int lane = threadIdx.x & 31;
-  if (unit >= (int64_t)a.n_seg * a.channels) return;
-  const int64_t s = unit / a.channels;
-  const int c = (int)(unit % a.channels);
   int64_t from, to;
   segment_rows(a, s, from, to);
   if (!by_chunks(a, to - from)) return;
-  float t1 = 0.f, t2 = 0.f;
-  if (from < to)
-    for (int64_t c0 = from / a.chunk + lane; c0 <= (to - 1) / a.chunk; c0 += 32 * 8) {
-      float2 v[8];
+  for (int c = blockIdx.y * GN_WARPS + (threadIdx.x >> 5); c < a.channels; c += gridDim.y * GN_WARPS) {
+    float t1 = 0.f, t2 = 0.f;
+    if (from < to)
+      for (int64_t c0 = from / a.chunk + lane; c0 <= (to - 1) / a.chunk; c0 += 32 * 8) {
+        float2 v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = c0 + 32 * i <= (to - 1) / a.chunk ? *reinterpret_cast<const float2*>(a.part + 2 * ((c0 + 32 * i + s) * a.channels + c))
-                                                 : make_float2(0.f, 0.f);
+        for (int i = 0; i < 8; ++i)
+          v[i] = c0 + 32 * i <= (to - 1) / a.chunk ? *reinterpret_cast<const float2*>(a.part + 2 * ((c0 + 32 * i + s) * a.channels + c))
+                                                   : make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { t1 += v[i].x; t2 += v[i].y; }
-    }
-  t1 = warp_sum(t1);
-  t2 = warp_sum(t2);
-  if (lane == 0) { a.sums[2 * unit] = t1; a.sums[2 * unit + 1] = t2; }
+        for (int i = 0; i < 8; ++i) { t1 += v[i].x; t2 += v[i].y; }
+      }
+    t1 = warp_sum(t1);
+    t2 = warp_sum(t2);
+    if (lane == 0) { a.sums[2 * (s * a.channels + c)] = t1; a.sums[2 * (s * a.channels + c) + 1] = t2; }
+  }
 }
 
 template <typename T, int V, int NC, bool ACT>
@@ -892,6 +891,10 @@ template <typename F> static void gn_typed(int dtype, bool vec, F f) {
   else if (dtype == MB_DTYPE_BF16) { if (vec) f.template operator()<__nv_bfloat16, 8, 1>(); else f.template operator()<__nv_bfloat16, 1, 4>(); }
   else { if (vec) f.template operator()<__half, 8, 1>(); else f.template operator()<__half, 1, 4>(); }
 }
+static dim3 gn_join_grid(int n_seg, int units) {  // some 1,024 blocks, a warp for every unit of one segment at the most
+  const int all = cdiv(units, GN_WARPS), want = 1024 / n_seg;
+  return dim3((unsigned)n_seg, (unsigned)(want < 1 ? 1 : want < all ? want : all));
+}
 struct GnFwdLaunch {
   const GnArgs& a; int n_sm; cudaStream_t st; bool blocks, chunks;
   template <typename T, int V, int NC> void operator()() const {
@@ -905,7 +908,7 @@ struct GnFwdLaunch {
     if (chunks) {
       const unsigned grid = (unsigned)cdiv(a.n_rows, a.chunk);
       launch(k_group_norm_part<T, V, NC>, grid, GN_THREADS, 0, st, a);
-      launch(k_group_norm_join, (unsigned)cdiv((int64_t)a.n_seg * a.groups, GN_WARPS), GN_THREADS, 0, st, a);
+      launch(k_group_norm_join, gn_join_grid(a.n_seg, a.groups), GN_THREADS, 0, st, a);
       if (a.act) launch(k_group_norm_apply<T, V, NC, true>, grid, GN_THREADS, 0, st, a);
       else launch(k_group_norm_apply<T, V, NC, false>, grid, GN_THREADS, 0, st, a);
     }
@@ -925,7 +928,7 @@ struct GnBwdLaunch {
     if (chunks) {
       const unsigned grid = (unsigned)cdiv(a.n_rows, a.chunk);
       launch(k_group_norm_bwd_part<T, V, NC, ACT>, grid, GN_THREADS, 0, st, a);
-      launch(k_group_norm_bwd_join, (unsigned)cdiv((int64_t)a.n_seg * a.channels, GN_WARPS), GN_THREADS, 0, st, a);
+      launch(k_group_norm_bwd_join, gn_join_grid(a.n_seg, a.channels), GN_THREADS, 0, st, a);
       launch(k_group_norm_bwd_apply<T, V, NC, ACT>, grid, GN_THREADS, 0, st, a);
     }
   }
