@@ -490,7 +490,7 @@ int mb_experts_grad_w(const mb_experts* d, void* stream);
 
 /* out[t] = sum_j weights[t,j] y[slot_of[t,j]] over the choices j with a slot (weights NULL: 1); width a multiple of 4, top_k <= 32.
  * bwd: dy[slot_of[t,j]] = weights[t,j] dout[t], dweights[t,j] = dout[t] . y[slot_of[t,j]] (0 without a slot; NULL: not wanted); dy rows
- * from offsets[n_experts] on are set to zero where offsets is given. */
+ * from offsets[n_experts] on are set to zero where offsets is given.  bwd wants every slot in slot_of once at the most. */
 typedef struct mb_combine {
   int64_t n_rows, n_slots;
   int32_t top_k, width, n_experts, pad0;

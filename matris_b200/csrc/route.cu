@@ -566,7 +566,7 @@ static int route_blocks(int64_t n_rows, int n_sm) {
 static bool route_small(int64_t n_rows, int n_experts) { return n_rows * n_experts <= 4096; }
 static bool route_valid(const mb_route* d) {
   return d && d->n_rows >= 0 && d->n_experts >= 1 && d->n_experts <= RT_MAX_EXPERTS && d->top_k >= 1 && d->top_k <= RT_MAX_K &&
-         d->top_k <= d->n_experts && d->dtype >= 0 && d->dtype <= 2 && d->n_rows * d->top_k <= INT32_MAX;
+         d->top_k <= d->n_experts && d->dtype >= 0 && d->dtype <= 2 && d->n_rows <= INT32_MAX / d->top_k;
 }
 static RtArgs route_args(const mb_route* d) {
   RtArgs a = {};
@@ -669,7 +669,7 @@ static bool rows16(const void* p, int64_t ld, int width) {
 }
 static bool combine_valid(const mb_combine* d) {
   return d && d->n_rows >= 0 && d->n_slots >= 0 && d->n_slots <= INT32_MAX && d->top_k >= 1 && d->top_k <= RT_MAX_K && d->width >= 4 && d->width % 4 == 0 &&
-         d->n_rows * d->top_k <= INT32_MAX && (d->n_rows == 0 || d->slot_of);
+         d->n_rows <= INT32_MAX / d->top_k && d->n_experts >= 0 && (d->n_rows == 0 || d->slot_of);
 }
 static CbArgs combine_args(const mb_combine* d) {
   CbArgs a = {};

@@ -800,6 +800,8 @@ def experts_grad_w(dy, x, offsets, idx=None, in_act=0, want_bias=True):
 
 def _combine_args(y, slot_of, weights):
     """Row stride and shape of the experts' outputs, rows and choices a row."""
+    if not isinstance(y, torch.Tensor):
+        raise TypeError(f"y: a tensor is wanted, got {type(y).__name__}")
     if y.dim() != 2:
         raise ValueError(f"y: [slots, width] is wanted, got shape {tuple(y.shape)}")
     if not isinstance(slot_of, torch.Tensor) or slot_of.dtype != _I32:
@@ -830,7 +832,8 @@ def experts_combine_fwd(y, slot_of, weights=None):
 
 def experts_combine_bwd(dout, y, slot_of, weights=None, offsets=None):
     """Gradients (dy, dweights) of ``experts_combine_fwd``: dy [slots, width], dweights [rows, top_k] (0 for a choice without a
-    slot).  Slots that no choice has are zero from ``offsets[-1]`` on; without ``offsets`` every slot has to have its choice."""
+    slot).  Slots that no choice has are zero from ``offsets[-1]`` on; without ``offsets`` every slot has to have its choice.  A slot
+    is one choice's, as in ``Route.slot_of``: two that name the same one would overwrite each other's dy."""
     ld, n_slots, width, n, k = _combine_args(y, slot_of, weights)
     ld_dout = _take_rows(dout, "dout", _F32, n, width, aligned=True)
     n_experts = 0

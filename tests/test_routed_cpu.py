@@ -97,6 +97,21 @@ def test_the_library_refuses(struct, name, fields, library):
     assert getattr(library, name)(None, None) == _lib.MB_ERR_INVALID
 
 
+@pytest.mark.parametrize("struct,name,fields", [
+    (_lib.MbRoute, "mb_route_fwd", dict(n_rows=1 << 60, n_experts=32, top_k=16, ld_logits=32)),  # 2^64 choices are 0 in 64 bits
+    (_lib.MbRoute, "mb_route_bwd", dict(n_rows=1 << 60, n_experts=32, top_k=16, ld_logits=32, ld_dlogits=32)),
+    (_lib.MbCombine, "mb_experts_combine_fwd", dict(n_rows=1 << 60, n_slots=4, top_k=16, width=8, ld_y=8, ld_out=8)),
+    (_lib.MbCombine, "mb_experts_combine_bwd", dict(n_rows=4, n_slots=4, top_k=2, width=8, n_experts=-1, ld_y=8, ld_dout=8, ld_dy=8)),
+])
+def test_the_library_refuses_sizes(struct, name, fields, library):
+    """All pointers given (and not looked at): the sizes alone are refused."""
+    d = struct(**fields)
+    for field, kind in struct._fields_:
+        if kind is C.c_void_p:
+            setattr(d, field, 1 << 12)
+    assert getattr(library, name)(C.byref(d), None) == _lib.MB_ERR_INVALID
+
+
 def test_struct_layouts_match_the_header(tmp_path):
     import os
     import subprocess
@@ -110,3 +125,8 @@ def test_struct_layouts_match_the_header(tmp_path):
     for line in subprocess.check_output([str(tmp_path / "t")], text=True).splitlines():
         n, *got = line.split()
         assert [int(v) for v in got] == [C.sizeof(names[n])] + [getattr(names[n], f[0]).offset for f in names[n]._fields_], n
+
+
+def test_combination_wants_tensors():
+    with pytest.raises(TypeError):
+        ops.experts_combine_fwd([1.0], torch.zeros(1, 1, dtype=I))
