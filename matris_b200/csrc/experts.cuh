@@ -302,6 +302,7 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
 #pragma unroll 1
           for (int cg = 0; cg < 4; ++cg) {
             uint32_t v[16], u[16];
+            __syncwarp();  // lanes without a row have skipped the previous columns' work; these reads want the whole warp
             MB_TMEM_LD16(lane_base + 16u * cg, v);
             MB_TMEM_LD16(lane_base + 128u + 16u * cg, u);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -401,6 +402,7 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
         for (int i = 0; i < 8; ++i) split_tf32_even(v[i], hi[i], lo[i]);
         if (h == 0) {
           if (n > 0 && alive) alive = mbar_wait(a_done + 8 * set, (n - 1) & 1);  // the A buffer is free again
+          alive = __all_sync(0xffffffffu, alive);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
         MB_TMEM_ST8(ta + 8 * h, hi);
