@@ -8,6 +8,8 @@ from __future__ import annotations
 import ctypes as C
 import math
 import struct
+import threading
+from collections import OrderedDict
 from typing import NamedTuple
 
 import torch
@@ -58,22 +60,29 @@ class SplitWeight:
         return SplitWeight(self.w.t())
 
 
-_split_cache: dict = {}
+_split_cache: OrderedDict = OrderedDict()  # used longest ago first
+_split_lock = threading.Lock()
+_SPLITS_KEPT = 257
 
 
 def as_split(W) -> SplitWeight:
+    """The operand splits of a weight, kept for the next call with it.  The caller holds what it gets until its launch is made:
+    another thread may make room in the meantime, and addresses alone keep nothing alive."""
     if isinstance(W, SplitWeight):
         return W
     # an entry keeps W, so that its address is not handed out again; views of one storage differ in shape or strides
     key = (W.data_ptr(), tuple(W.shape), W.stride(), W._version)
-    entry = _split_cache.pop(key, None)
-    if entry is None:
-        # the one used longest ago goes: never one that the call in progress has just looked up
-        if len(_split_cache) > 256:
-            del _split_cache[next(iter(_split_cache))]
-        entry = (W.detach(), SplitWeight(W))
-    _split_cache[key] = entry
-    return entry[1]
+    with _split_lock:
+        entry = _split_cache.get(key)
+        if entry is not None:
+            _split_cache.move_to_end(key)
+            return entry[1]
+    split = SplitWeight(W)
+    with _split_lock:
+        _split_cache.setdefault(key, (W.detach(), split))  # of threads that built it at once, the first one's stays
+        while len(_split_cache) > _SPLITS_KEPT:
+            _split_cache.popitem(last=False)
+    return split
 
 
 def S(t, idx=None, col=0, act=0):
@@ -108,6 +117,7 @@ def gemm(n_rows: int, blocks: list[dict]) -> None:
     buf = bytearray(_DESC_SIZE)
     _HDR_FMT.pack_into(buf, 0, n_rows, len(blocks), 0)
     off = _BLK_OFF
+    held = []  # splits looked up here, until the launch is made
     last_srcs = flat = None
     for b in blocks:
         srcs = b["srcs"]
@@ -122,6 +132,7 @@ def gemm(n_rows: int, blocks: list[dict]) -> None:
         sw = b["W"]
         if type(sw) is not SplitWeight:
             sw = as_split(sw)
+            held.append(sw)
         ldw = sw.ldw
         assert sw.shape[1] >= D * n_src
         w_off = 4 * ldw * b["w_row"]
@@ -253,7 +264,8 @@ def mlp_bwd(dy, w2t, w1t, z1, gated, want_dz1=True, res=None, res_w=None, idx=No
     m = _lib.MbMlpBwd()
     m.n_rows, m.kind, m.scale = n_rows, 0 if gated else 1, scale
     m.dy = _lib.MbSrc(dy.data_ptr(), 0 if idx is None else idx.data_ptr(), dy.stride(0), 0, 0)
-    m.W2t, m.W1t = (_lib.MbWeight(*s.ptrs, s.ldw) for s in (as_split(w2t), as_split(w1t)))
+    w2, w1 = as_split(w2t), as_split(w1t)
+    m.W2t, m.W1t = (_lib.MbWeight(*s.ptrs, s.ldw) for s in (w2, w1))
     if ext is not None:
         m.n_ext = ext.shape[1] // D
         for j in range(m.n_ext):
