@@ -61,23 +61,32 @@ class SplitWeight:
 
 
 _split_cache: OrderedDict = OrderedDict()  # used longest ago first
+_split_graphs: dict = {}  # entries that captured graphs read: these stay
 _split_lock = threading.Lock()
 _SPLITS_KEPT = 257
 
 
 def as_split(W) -> SplitWeight:
     """The operand splits of a weight, kept for the next call with it.  The caller holds what it gets until its launch is made:
-    another thread may make room in the meantime, and addresses alone keep nothing alive."""
+    another thread may make room in the meantime, and addresses alone keep nothing alive.
+
+    In a capture, splits that were there before stay for good, since the graph may be replayed at any time; others become part of the
+    graph and are nobody else's, for they hold values only when it has run."""
     if isinstance(W, SplitWeight):
         return W
     # an entry keeps W, so that its address is not handed out again; views of one storage differ in shape or strides
     key = (W.data_ptr(), tuple(W.shape), W.stride(), W._version)
+    capturing = W.is_cuda and torch.cuda.is_current_stream_capturing()
     with _split_lock:
         entry = _split_cache.get(key)
         if entry is not None:
             _split_cache.move_to_end(key)
+            if capturing:
+                _split_graphs[key] = entry
             return entry[1]
     split = SplitWeight(W)
+    if capturing:
+        return split
     with _split_lock:
         _split_cache.setdefault(key, (W.detach(), split))  # of threads that built it at once, the first one's stays
         while len(_split_cache) > _SPLITS_KEPT:
