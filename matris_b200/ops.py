@@ -60,6 +60,22 @@ class SplitWeight:
         return SplitWeight(self.w.t())
 
 
+class _Kept(NamedTuple):
+    weight: torch.Tensor   # so that its address is not handed out again
+    split: SplitWeight
+    built: object          # event behind the splits' kernels (None on the CPU)
+    streams: set           # raw handles of the streams that are ordered behind it
+
+    def reach(self, stream: int) -> None:
+        """Before the first use on another stream than the one that built the splits: it waits for them, and their memory is not
+        handed out again before it has read them."""
+        here = torch.cuda.current_stream()
+        here.wait_event(self.built)
+        for t in (self.split.w, self.split.hi, self.split.lo, self.split.hi16, self.split.lo16):
+            t.record_stream(here)
+        self.streams.add(stream)
+
+
 _split_cache: OrderedDict = OrderedDict()  # used longest ago first
 _split_graphs: dict = {}  # entries that captured graphs read: these stay
 _split_lock = threading.Lock()
@@ -67,28 +83,32 @@ _SPLITS_KEPT = 257
 
 
 def as_split(W) -> SplitWeight:
-    """The operand splits of a weight, kept for the next call with it.  The caller holds what it gets until its launch is made:
-    another thread may make room in the meantime, and addresses alone keep nothing alive.
+    """The operand splits of a weight, kept for the next call with it on any stream.  The caller holds what it gets until its launch
+    is made: another thread may make room in the meantime, and addresses alone keep nothing alive.
 
     In a capture, splits that were there before stay for good, since the graph may be replayed at any time; others become part of the
     graph and are nobody else's, for they hold values only when it has run."""
     if isinstance(W, SplitWeight):
         return W
-    # an entry keeps W, so that its address is not handed out again; views of one storage differ in shape or strides
+    # views of one storage differ in shape or strides
     key = (W.data_ptr(), tuple(W.shape), W.stride(), W._version)
-    capturing = W.is_cuda and torch.cuda.is_current_stream_capturing()
+    stream = _stream() if W.is_cuda else 0
+    capturing = stream != 0 and torch.cuda.is_current_stream_capturing()
     with _split_lock:
         entry = _split_cache.get(key)
         if entry is not None:
             _split_cache.move_to_end(key)
             if capturing:
                 _split_graphs[key] = entry
-            return entry[1]
+            elif stream not in entry.streams:
+                entry.reach(stream)
+            return entry.split
     split = SplitWeight(W)
     if capturing:
         return split
+    entry = _Kept(W.detach(), split, torch.cuda.current_stream().record_event() if W.is_cuda else None, {stream})
     with _split_lock:
-        _split_cache.setdefault(key, (W.detach(), split))  # of threads that built it at once, the first one's stays
+        _split_cache.setdefault(key, entry)  # of threads that built it at once, the first one's stays
         while len(_split_cache) > _SPLITS_KEPT:
             _split_cache.popitem(last=False)
     return split
