@@ -465,7 +465,8 @@ int mb_route_bwd(const mb_route* d, void* stream);
 /* The experts' dense layers on grouped rows: slot s of expert e (offsets[e] <= s < offsets[e+1])
  *   y[s] = act(f(x[idx[s]]) W_e^T + bias_e) [* SiLU'(gate[s])]       W [n_experts, n_out, n_in], bias [n_experts, n_out]
  * idx NULL: row s itself; in_act: f = SiLU.  Widths are multiples of 128, at most 1024; rows 16-byte aligned.
- * Slots behind offsets[n_experts] are left as they are, or set to zero with zero_rest.  Offsets and idx are cut to their ranges.
+ * Slots ahead of offsets[0] (a share of the experts: a part of a grouping's offsets) and from offsets[n_experts] on are left as they
+ * are, or set to zero with zero_rest.  Offsets and idx are cut to their ranges.
  * The data gradient is the same call on the transposed parts, n_in and n_out exchanged.
  * split: parts [4, n_experts * n_out * n_in] = hi and lo of w (w = hi + lo, hi of 11 significant bits), hi and lo of every expert's
  * transpose [n_in, n_out]; 16-byte aligned.
@@ -489,8 +490,10 @@ size_t mb_experts_grad_scratch(int64_t n_slots, int32_t n_experts, int32_t n_in,
 int mb_experts_grad_w(const mb_experts* d, void* stream);
 
 /* out[t] = sum_j weights[t,j] y[slot_of[t,j]] over the choices j with a slot (weights NULL: 1); width a multiple of 4, top_k <= 32.
- * bwd: dy[slot_of[t,j]] = weights[t,j] dout[t], dweights[t,j] = dout[t] . y[slot_of[t,j]] (0 without a slot; NULL: not wanted); dy rows
- * from offsets[n_experts] on are set to zero where offsets is given.  bwd wants every slot in slot_of once at the most. */
+ * bwd: dy[slot_of[t,j]] = weights[t,j] dout[t], dweights[t,j] = dout[t] . y[slot_of[t,j]] (0 without a slot; NULL: not wanted).  Where
+ * offsets is given, slots ahead of offsets[0] and from offsets[n_experts] on are no choice's: their dy rows are set to zero, and a choice
+ * that names one counts as without a slot.  Other dy rows that no choice names are left as they are.  bwd wants every slot in slot_of
+ * once at the most. */
 typedef struct mb_combine {
   int64_t n_rows, n_slots;
   int32_t top_k, width, n_experts, pad0;

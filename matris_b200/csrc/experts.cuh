@@ -416,10 +416,13 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
 
-  if (d.zero_rest) {  // slots behind the last
-    const int64_t used = min(max((int64_t)d.offsets[d.n_experts], (int64_t)0), d.n_slots);
-    for (int64_t s = used + (int64_t)blockIdx.x * (EX_THREADS / 32) + warp; s < d.n_slots; s += (int64_t)gridDim.x * (EX_THREADS / 32))
+  if (d.zero_rest) {  // slots ahead of the first expert's and behind the last one's
+    const int64_t first = min(max((int64_t)d.offsets[0], (int64_t)0), d.n_slots);
+    const int64_t used = min(max((int64_t)d.offsets[d.n_experts], first), d.n_slots), skip = used - first;
+    for (int64_t i = (int64_t)blockIdx.x * (EX_THREADS / 32) + warp; i < d.n_slots - skip; i += (int64_t)gridDim.x * (EX_THREADS / 32)) {
+      const int64_t s = i < first ? i : i + skip;
       for (int c = 4 * lane; c < d.n_out; c += 128) st4(d.y + s * d.ld_y + c, make_float4(0.f, 0.f, 0.f, 0.f));
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();

@@ -495,13 +495,13 @@ __global__ void __launch_bounds__(RT_THREADS) k_combine(const __grid_constant__ 
 struct Choices {
   int slot;     // -1: none
   float w;
-  __device__ __forceinline__ void ask(const CbArgs& a, int64_t t, int lane) {
+  __device__ __forceinline__ void ask(const CbArgs& a, int64_t t, int lane, int64_t first, int64_t used) {
     slot = -1;
     w = 1.f;
     if (t < a.n_rows && lane < a.top_k) {
       slot = a.slot_of[t * a.top_k + lane];
       if (a.weights) w = a.weights[t * a.top_k + lane];
-      if (slot >= a.n_slots) slot = -1;
+      if (slot < first || slot >= used) slot = -1;
     }
   }
 };
@@ -510,16 +510,21 @@ __global__ void __launch_bounds__(RT_THREADS) k_combine_bwd(const __grid_constan
   pdl_sync();
   const int lane = threadIdx.x & 31;
   const int64_t step = (int64_t)gridDim.x * RT_WARPS, t0 = (int64_t)blockIdx.x * RT_WARPS + (threadIdx.x >> 5);
-  if (a.offsets) {  // rows of no slot
-    const int64_t used = max(a.offsets[a.n_experts], 0);
-    for (int64_t s = used + t0; s < a.n_slots; s += step)
+  int64_t first = 0, used = a.n_slots;  // slots of the experts; the others are no choice's, whoever names them
+  if (a.offsets) {
+    first = min(max((int64_t)a.offsets[0], (int64_t)0), a.n_slots);
+    used = min(max((int64_t)a.offsets[a.n_experts], first), a.n_slots);
+    const int64_t skip = used - first;
+    for (int64_t i = t0; i < a.n_slots - skip; i += step) {
+      const int64_t s = i < first ? i : i + skip;
       for (int c = 4 * lane; c < a.width; c += 128) st4(a.dy + s * a.ld_dy + c, make_float4(0.f, 0.f, 0.f, 0.f));
+    }
   }
   Choices next;
-  next.ask(a, t0, lane);
+  next.ask(a, t0, lane, first, used);
   for (int64_t t = t0; t < a.n_rows; t += step) {
     const Choices now = next;
-    next.ask(a, t + step, lane);
+    next.ask(a, t + step, lane, first, used);
     float mine = 0.f;  // lane j: dweights[t, j]
     for (int j0 = 0; j0 < a.top_k; j0 += 4) {
       float dot[4] = {0.f, 0.f, 0.f, 0.f};

@@ -792,7 +792,8 @@ def experts_linear(x, weights, offsets, bias=None, idx=None, in_act=0, out_act=0
 
     ``weights``: ExpertWeights, or a [experts, n_out, n_in] tensor that is laid out in the call; ``transposed``: W_e in the place
     of its transpose, the data gradient.  ``in_act`` / ``out_act`` 1: SiLU.  ``offsets``, ``idx``: ``Route.offsets``, ``Route.row_of``.
-    Slots behind the last are zero in a returned tensor and left alone in a given ``out``, which must not overlap the inputs."""
+    A part of a grouping's offsets with the weights of those experts is a share of the work.  Slots of no expert, ahead of ``offsets[0]`` and
+    from ``offsets[-1]`` on, are zero in a returned tensor and left alone in a given ``out``, which must not overlap the inputs."""
     if not isinstance(weights, ExpertWeights):
         weights = ExpertWeights(weights)
     n_experts, n_out, n_in = weights.shape
@@ -873,7 +874,8 @@ def experts_combine_fwd(y, slot_of, weights=None):
 
 def experts_combine_bwd(dout, y, slot_of, weights=None, offsets=None):
     """Gradients (dy, dweights) of ``experts_combine_fwd``: dy [slots, width], dweights [rows, top_k] (0 for a choice without a
-    slot).  Slots that no choice has are zero from ``offsets[-1]`` on; without ``offsets`` every slot has to have its choice.  A slot
+    slot).  With ``offsets``, every slot from ``offsets[0]`` to ``offsets[-1]`` - 1 has to have its choice, as in a Route; the others are
+    zero in dy and count as no slot.  Without, every slot has to have its choice.  A slot
     is one choice's, as in ``Route.slot_of``: two that name the same one would overwrite each other's dy."""
     ld, n_slots, width, n, k = _combine_args(y, slot_of, weights)
     ld_dout = _take_rows(dout, "dout", _F32, n, width, aligned=True)
@@ -883,7 +885,8 @@ def experts_combine_bwd(dout, y, slot_of, weights=None, offsets=None):
         if n_experts < 0:
             raise ValueError("offsets: [experts + 1] is wanted, got none")
     device = _here(dout, y, slot_of, weights, offsets)
-    dy, dweights = torch.empty((n_slots, width), dtype=_F32, device=y.device), torch.empty((n, k), dtype=_F32, device=y.device)
+    dy = torch.empty((n_slots, width), dtype=_F32, device=y.device)
+    dweights = torch.empty((n, k), dtype=_F32, device=y.device)
     _launch("mb_experts_combine_bwd", _lib.MbCombine, _COMBINE_FMT.pack(
         n, n_slots, k, width, n_experts, 0, slot_of.data_ptr(), ptr(offsets) or 0, ptr(weights) or 0, y.data_ptr(), ld, 0, 0, dout.data_ptr(),
         ld_dout, dy.data_ptr(), width, dweights.data_ptr()), device)
