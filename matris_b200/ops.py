@@ -875,7 +875,7 @@ def experts_combine_fwd(y, slot_of, weights=None):
 def experts_combine_bwd(dout, y, slot_of, weights=None, offsets=None):
     """Gradients (dy, dweights) of ``experts_combine_fwd``: dy [slots, width], dweights [rows, top_k] (0 for a choice without a
     slot).  With ``offsets``, every slot from ``offsets[0]`` to ``offsets[-1]`` - 1 has to have its choice, as in a Route; the others are
-    zero in dy and count as no slot.  Without, every slot has to have its choice.  A slot
+    zero in dy and count as no slot.  Without, dy is cleared first, so that slots that no choice has are zero.  A slot
     is one choice's, as in ``Route.slot_of``: two that name the same one would overwrite each other's dy."""
     ld, n_slots, width, n, k = _combine_args(y, slot_of, weights)
     ld_dout = _take_rows(dout, "dout", _F32, n, width, aligned=True)
@@ -885,7 +885,7 @@ def experts_combine_bwd(dout, y, slot_of, weights=None, offsets=None):
         if n_experts < 0:
             raise ValueError("offsets: [experts + 1] is wanted, got none")
     device = _here(dout, y, slot_of, weights, offsets)
-    dy = torch.empty((n_slots, width), dtype=_F32, device=y.device)
+    dy = (torch.zeros if offsets is None else torch.empty)((n_slots, width), dtype=_F32, device=y.device)
     dweights = torch.empty((n, k), dtype=_F32, device=y.device)
     _launch("mb_experts_combine_bwd", _lib.MbCombine, _COMBINE_FMT.pack(
         n, n_slots, k, width, n_experts, 0, slot_of.data_ptr(), ptr(offsets) or 0, ptr(weights) or 0, y.data_ptr(), ld, 0, 0, dout.data_ptr(),

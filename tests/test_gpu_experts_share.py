@@ -90,3 +90,15 @@ def test_shares_add_up_to_the_whole():
     # two terms a row, in the same order or the other one, each rounded as before: one more rounding of the sum
     assert ((total - whole).abs() <= 4 * 2.0 ** -24 * (total.abs() + whole.abs()) + 2.0 ** -22 * whole.abs().max()).all()
 
+
+def test_gradient_of_slots_that_no_choice_has_without_offsets():
+    from matris_b200 import ops
+    offsets, _, slot_of = grouped(50, 4, 2, 3)
+    slot_of = slot_of.clone()
+    slot_of[7], slot_of[20, 1] = -1, -1
+    y, dout = torch.randn(130, 128, device="cuda"), torch.randn(50, 128, device="cuda")
+    dirty(130, 128)
+    dy, _ = ops.experts_combine_bwd(dout, y, slot_of)
+    named = torch.zeros(130, dtype=torch.bool, device="cuda")
+    named[slot_of[slot_of >= 0].long()] = True
+    assert not dy[~named].any() and (dy[named] != 0).any(1).all()
