@@ -468,8 +468,10 @@ int mb_route_bwd(const mb_route* d, void* stream);
  * Slots ahead of offsets[0] (a share of the experts: a part of a grouping's offsets) and from offsets[n_experts] on are left as they
  * are, or set to zero with zero_rest.  Offsets and idx are cut to their ranges.
  * The data gradient is the same call on the transposed parts, n_in and n_out exchanged.
- * split: parts [4, n_experts * n_out * n_in] = hi and lo of w (w = hi + lo, hi of 11 significant bits), hi and lo of every expert's
- * transpose [n_in, n_out]; 16-byte aligned.
+ * Infinities in one operand and NaN give what they give in float32, in the products and in grad_w; an infinite value times an infinite or a
+ * subnormal one gives NaN.
+ * split: parts [4, n_experts * n_out * n_in] = hi and lo of w (w = hi + lo, hi of 11 significant bits, 0 for an infinite w), hi and lo of
+ * every expert's transpose [n_in, n_out]; 16-byte aligned.
  * grad_w: dw_e = sum_s dy[s]^T f(x[idx[s]]), dbias_e = sum_s dy[s] (dbias NULL: not wanted), summed in a fixed order. */
 typedef struct mb_experts {
   int64_t n_slots, n_rows;                                /* n_rows: rows of x */

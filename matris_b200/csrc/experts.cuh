@@ -145,9 +145,36 @@ static_assert(EX_SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
 
 // x = hi + lo, hi rounded to 11 significant bits by integer arithmetic (the conversion instruction runs at an eighth of the rate: two of
 // them a value took 512 cycles of the 768 that a chunk's products need).  The tensor cores read lo's leading 11 bits, of |lo| <= 2^-12 |x|.
-__device__ __forceinline__ void split_tf32_even(float x, uint32_t& hi, uint32_t& lo) {
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
+}
+// Eight values; `seen` gathers their lo: no longer finite once hi has been rounded out of the finite numbers, at half an instruction a value.
+__device__ __forceinline__ void split_tf32_all(const float (&x)[8], uint32_t (&hi)[8], uint32_t (&lo)[8], f2& seen) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) split_tf32(x[i], hi[i], lo[i]);
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) seen = seen + two(__uint_as_float(lo[i]), __uint_as_float(lo[i + 1]));
+}
+// Whether any lane of the warp has to split its chunk again by split_tf32_large.  (The weight gradient of 573,894 slots, 256 -> 128: 298 us
+// without the look, 308 so, 341 with a look at every eight values.)
+__device__ __forceinline__ bool split_again(f2 seen) {
+  float a, b;
+  apart(seen, a, b);
+  return __any_sync(0xffffffffu, !(fabsf(a + b) <= FLT_MAX));
+}
+// Next to 2^128 a finite x is cut instead of rounded; an infinity is left to lo, whose one product kept, with the other operand's hi, has
+// the right sign.  (As hi it would meet the other operand's lo too, which is of either sign or zero: NaN.)
+__device__ __forceinline__ void split_tf32_large(const float (&x)[8], uint32_t (&hi)[8], uint32_t (&lo)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = __float_as_uint(x[i]), size = u & 0x7FFFFFFFu;
+    if (size < 0x7F7FF000u) split_tf32(x[i], hi[i], lo[i]);
+    else {
+      hi[i] = size < 0x7F800000u ? u & 0xFFFFE000u : 0u;
+      lo[i] = __float_as_uint(x[i] - __uint_as_float(hi[i]));
+    }
+  }
 }
 
 __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant__ mb_experts d, const __grid_constant__ ExMaps maps, const int shared) {
@@ -388,18 +415,21 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
       asm volatile("cp.async.wait_group %0;" :: "n"(EX_STAGES - 1) : "memory");
       __syncwarp();
       const uint32_t patch = patch0 + (uint32_t)(n % EX_STAGES) * (32 * 128), ta = lane_base + 256 + 64 * set;
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        float v[8];
+      auto values = [&](int h, float (&v)[8]) {  // a quarter of this row's 32
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float4 f = lds4(patch + lane * 128 + (((2 * h + i) ^ (lane & 7)) << 4));
           v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
         }
         if (d.in_act) silu_fast_all(v, v);
-        uint32_t hi[8], lo[8];
+      };
+      f2 seen = two(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) split_tf32_even(v[i], hi[i], lo[i]);
+      for (int h = 0; h < 4; ++h) {
+        float v[8];
+        values(h, v);
+        uint32_t hi[8], lo[8];
+        split_tf32_all(v, hi, lo, seen);
         if (h == 0) {
           if (n > 0 && alive) alive = mbar_wait(a_done + 8 * set, (n - 1) & 1);  // the A buffer is free again
           alive = __all_sync(0xffffffffu, alive);
@@ -407,6 +437,19 @@ __global__ void __launch_bounds__(EX_THREADS, 1) k_experts(const __grid_constant
         }
         MB_TMEM_ST8(ta + 8 * h, hi);
         MB_TMEM_ST8(ta + 32 + 8 * h, lo);
+      }
+      if (split_again(seen)) {
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");  // the parts above are written over
+#pragma unroll 1
+        for (int h = 0; h < 4; ++h) {
+          float v[8];
+          values(h, v);
+          uint32_t hi[8], lo[8];
+          split_tf32_large(v, hi, lo);
+          __syncwarp();
+          MB_TMEM_ST8(ta + 8 * h, hi);
+          MB_TMEM_ST8(ta + 32 + 8 * h, lo);
+        }
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -442,7 +485,12 @@ __global__ void __launch_bounds__(256) k_experts_split(int n_out, int n_in, int6
 #pragma unroll
   for (int i = ty; i < 32; i += 8) {
     const int64_t at = e0 + (int64_t)(n0 + i) * n_in + k0 + tx;
-    const float x = w[at], hi = to_tf32(x), lo = to_tf32(x - hi);
+    const float x = w[at];
+    float hi = to_tf32(x), lo = to_tf32(x - hi);
+    if (!(fabsf(hi) <= FLT_MAX)) {  // as in split_tf32_large
+      hi = fabsf(x) <= FLT_MAX ? __uint_as_float(__float_as_uint(x) & 0xFFFFE000u) : 0.f;
+      lo = to_tf32(x - hi);
+    }
     parts[at] = hi;
     parts[part + at] = lo;
     t[0][i][tx] = hi;
@@ -674,16 +722,12 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
       alive = __all_sync(0xffffffffu, alive);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t line = tiles + b * 2 * TC_TILE_BYTES + col * 128;
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        uint32_t hi[8], lo[8];
-        float x[8];
+      auto values = [&](int h, float (&x)[8]) {  // a quarter of this column's 32
 #pragma unroll
         for (int i = 0; i < 8; ++i) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x[i]) : "r"(patch + 128u * (8 * h + i)) : "memory");
         if (is_x && d.in_act) silu_fast_all(x, x);
-        if (!is_x) bias += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) split_tf32_even(x[i], hi[i], lo[i]);
+      };
+      auto put = [&](int h, const uint32_t (&hi)[8], const uint32_t (&lo)[8]) {
         if (is_x) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -696,6 +740,28 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
         } else {
           MB_TMEM_ST8(lane_base + 64 * b + 8 * h, hi);
           MB_TMEM_ST8(lane_base + 64 * b + 32 + 8 * h, lo);
+        }
+      };
+      f2 seen = two(0.f, 0.f);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        uint32_t hi[8], lo[8];
+        float x[8];
+        values(h, x);
+        if (!is_x) bias += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        split_tf32_all(x, hi, lo, seen);
+        put(h, hi, lo);
+      }
+      if (split_again(seen)) {
+        if (!is_x) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");  // the parts above are written over
+#pragma unroll 1
+        for (int h = 0; h < 4; ++h) {
+          uint32_t hi[8], lo[8];
+          float x[8];
+          values(h, x);
+          split_tf32_large(x, hi, lo);
+          __syncwarp();
+          put(h, hi, lo);
         }
       }
       if (is_x) {

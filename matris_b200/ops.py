@@ -792,6 +792,7 @@ def experts_linear(x, weights, offsets, bias=None, idx=None, in_act=0, out_act=0
 
     ``weights``: ExpertWeights, or a [experts, n_out, n_in] tensor that is laid out in the call; ``transposed``: W_e in the place
     of its transpose, the data gradient.  ``in_act`` / ``out_act`` 1: SiLU.  ``offsets``, ``idx``: ``Route.offsets``, ``Route.row_of``.
+    Infinities in one operand and NaN give what they give in float32; infinite times infinite or subnormal values give NaN.
     A part of a grouping's offsets with the weights of those experts is a share of the work.  Slots of no expert, ahead of ``offsets[0]`` and
     from ``offsets[-1]`` on, are zero in a returned tensor and left alone in a given ``out``, which must not overlap the inputs."""
     if not isinstance(weights, ExpertWeights):

@@ -16,7 +16,7 @@ def test_warps_are_whole_where_they_reach_tensor_memory():
     warp comes first."""
     text = code("experts.cuh")
     found = accesses(text)
-    assert len(found) == 7
+    assert len(found) == 9
     for at in found:
         wait = text.rfind("mbar_wait(", 0, at)
         assert re.search(r"__all_sync\(|__syncwarp\(\)", text[wait:at]), text[wait:at]
