@@ -518,13 +518,14 @@ __global__ void __launch_bounds__(256) k_experts_split(int n_out, int n_in, int6
 //
 // The tensor cores cut each sum they accumulate to float32 instead of rounding it, always towards zero: after n of them a sum is
 // short by up to n 2^-23.  So a run is accumulated there for EG_FLUSH chunks only and added up in float32 registers of the epilogue
-// warps, rounded to nearest.
+// warps, rounded to nearest; after EG_FOLD such sums, 4,096 rows, these go to their place in memory and start again, so that no chain of
+// additions grows with the number of rows but that of the 4,096s (the bias gradient's are added in 64 bits).
 //
 // 573,894 slots, 256 -> 128, 32 experts: 297 us (127 TFLOP/s).  The column warps bound it, some 2,000 cycles a chunk of their own
 // instructions where its products take 768; sixteen of them do not fit the registers beside the epilogue's sums.
 //
 // Roles: warp 0 issues the products, warps 2 - 5 hold dy's columns, 6 - 9 x's, 10 - 17 the sums (warp 1 has none).
-constexpr int EG_FLUSH = 4;
+constexpr int EG_FLUSH = 4, EG_FOLD = 32;
 constexpr int EG_BUFS = 4;
 constexpr int EG_STAGES = 3;
 constexpr int EG_PATCH_OFF = EG_BUFS * 2 * TC_TILE_BYTES;
@@ -543,8 +544,8 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + EG_BAR_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + EG_BAR_OFF + 240);
-  // of an accumulator: -3 the run goes on, -2 / -1 it ends and is the share's first / second partial sum, e >= 0: all of expert e;
-  // -4: the share is done
+  // of an accumulator: -3: the run goes on; otherwise the run's sum goes to place (what >> 1) - 2, added to what it has left there before, and
+  // ends with what & 1.  Place -2 / -1: the share's first / second partial sum, e >= 0: all of expert e.  -4: the share is done
   volatile int32_t* const target = reinterpret_cast<volatile int32_t*>(smem + EG_BAR_OFF + 224);
   if ((smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0) atomicOr(&g_gemm_status, 2);
@@ -588,7 +589,7 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
     uint32_t elected;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0), tiles_u = __shfl_sync(0xffffffffu, tiles, 0);
-    uint32_t g = 0, k = 0, in_acc = 0;
+    uint32_t g = 0, k = 0, in_acc = 0, sums = 0;  // sums of the run in the epilogue's registers
     bool fresh = true, from_start = false;
     auto tell = [&](int32_t what) {
       if (lane == 0) {
@@ -606,7 +607,16 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const bool end = left <= 32 || t + 1 == share.hi;
       const bool flush = in_acc == EG_FLUSH - 1 || end;
-      if (flush) tell(!end ? -3 : from_start && left <= 32 ? e : from_start ? -1 : -2);
+      if (flush) {
+        ++sums;
+        if (end || sums == EG_FOLD) {
+          const bool all = from_start && left <= 32 * (share.hi - t);  // the expert ends in this share too
+          tell(2 * ((all ? e : from_start ? -1 : -2) + 2) + (end ? 1 : 0));
+          sums = 0;
+        } else {
+          tell(-3);
+        }
+      }
       // from one lane, so that the operands of the matrix instructions are the same for all by construction (see k_experts)
       const uint32_t how = __shfl_sync(0xffffffffu, b | acc << 2 | (in_acc == 0 ? 8u : 0u) | (flush ? 16u : 0u), 0);
       const uint32_t ub = how & 3, uacc = how >> 2 & 1;
@@ -631,6 +641,7 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
     f2 sum[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) sum[i] = two(0.f, 0.f);
+    bool more = false;  // this run has left a sum at its place before
     for (uint32_t k = 0; ; ++k) {
       const uint32_t acc = k & 1;
       if (alive) alive = mbar_wait(told + 8 * acc, (k >> 1) & 1);
@@ -652,15 +663,18 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
       __syncwarp();
       if (lane == 0) mbar_arrive(d_free + 8 * acc);
       if (what == -3) continue;
-      float* const out = (what >= 0 ? d.dw + what * whole : part + (2 * c + 2 + what) * whole) + at;
+      const int place = (what >> 1) - 2;
+      float* const out = (place >= 0 ? d.dw + place * whole : part + (2 * c + 2 + place) * whole) + at;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float o[4];
         apart(sum[2 * i], o[0], o[1]);
         apart(sum[2 * i + 1], o[2], o[3]);
+        if (more) add4_to(o, ld4(out + 4 * i));
         if (alive) st4(out + 4 * i, make_float4(o[0], o[1], o[2], o[3]));
         sum[2 * i] = sum[2 * i + 1] = two(0.f, 0.f);
       }
+      more = !(what & 1);
     }
   } else if (warp >= PS_PROD_WARP0) {
     // columns: warps 2 - 5 dy (A, tensor memory), 6 - 9 x (B, shared memory), 32 columns each
@@ -711,6 +725,8 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
     if (!is_x) { now.start(d); }
     uint32_t g = 0;
     float bias = 0.f;
+    double bias_sum = 0.;
+    int summed = 0;  // chunks in `bias`
     bool fresh = true, from_start = false;
     for (int64_t t = share.lo; t < share.hi; ++t, ++g) {
       const uint32_t b = g & 3;
@@ -770,12 +786,18 @@ k_experts_grad(const __grid_constant__ mb_experts d, const int n_share, float* c
         now.next((int)t, e0, now_s, now_left, first0);
         const bool last0 = now_left <= 32;
         if (fresh) { from_start = first0; fresh = false; }
-        if (last0 || t + 1 == share.hi) {
+        const bool end = last0 || t + 1 == share.hi;
+        if (++summed == EG_FOLD * EG_FLUSH || end) {
+          bias_sum += (double)bias;
+          bias = 0.f;
+          summed = 0;
+        }
+        if (end) {
           if (part_bias && k0 == 0) {
             float* const out = from_start && last0 ? d.dbias + (int64_t)e0 * d.n_out : part_bias + (int64_t)(2 * c + (from_start ? 1 : 0)) * d.n_out;
-            out[n0 + col] = bias;
+            out[n0 + col] = (float)bias_sum;
           }
-          bias = 0.f;
+          bias_sum = 0.;
           fresh = true;
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
