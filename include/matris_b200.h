@@ -456,7 +456,7 @@ typedef struct mb_route {
   int32_t *offsets, *row_of, *slot_of;
   const float *dweights, *dloss;
   void* dlogits; int64_t ld_dlogits;
-  void* scratch;                                          /* fwd: mb_route_scratch() bytes (0: NULL will do) */
+  void* scratch;                                          /* fwd: mb_route_scratch() bytes (0: NULL will do), 16-byte aligned */
 } mb_route;
 size_t mb_route_scratch(int64_t n_rows, int32_t n_experts);
 int mb_route_fwd(const mb_route* d, void* stream);
@@ -484,7 +484,7 @@ typedef struct mb_experts {
   float* y; int64_t ld_y;
   const float* dy; int64_t ld_dy;
   float* dw; float* dbias;
-  void* scratch;                                          /* grad_w: mb_experts_grad_scratch() bytes */
+  void* scratch;                                          /* grad_w: mb_experts_grad_scratch() bytes, 16-byte aligned */
 } mb_experts;
 int mb_experts_split(int32_t n_experts, int32_t n_out, int32_t n_in, const float* w, float* parts, void* stream);
 int mb_experts_linear(const mb_experts* d, void* stream);

@@ -844,6 +844,7 @@ static bool gn_valid(const mb_group_norm* d) {
   if (!d || d->n_rows < 0 || d->n_seg < 0 || d->channels < 1 || d->channels > GN_MAX_CHANNELS || d->groups < 1) return false;
   if (d->channels % d->groups || d->dtype < 0 || d->dtype > 2 || d->act < 0 || d->act > 1 || !(d->eps > 0.f)) return false;
   if (!d->seg_ptr && d->n_seg > 0 && d->n_rows % d->n_seg) return false;
+  if (reinterpret_cast<uintptr_t>(d->scratch) & 15u) return false;
   return d->n_rows <= INT32_MAX;
 }
 // Rows of a chunk: as many as put one block into each of GN_PLACES places of every multiprocessor, so that they all run at once.  (Every chunk

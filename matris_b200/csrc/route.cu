@@ -636,7 +636,7 @@ extern "C" int mb_route_fwd(const mb_route* d, void* stream) {
   if (d->n_rows > 0 && (!d->logits || d->ld_logits < d->n_experts || !d->ids || !d->weights || !d->row_of || !d->slot_of))
     return MB_ERR_INVALID;
   const bool small = route_small(d->n_rows, d->n_experts);
-  if (!small && !d->scratch) return MB_ERR_INVALID;
+  if (!small && (!d->scratch || (reinterpret_cast<uintptr_t>(d->scratch) & 15u))) return MB_ERR_INVALID;
   const cudaStream_t st = (cudaStream_t)stream;
   int n_sm = 0, rc = sm_count(&n_sm);
   if (rc) return rc;
