@@ -25,7 +25,7 @@ __device__ __forceinline__ const float* source_row(const mb_experts& d, int64_t 
 // most 2^-24 of |x w| and of either sign: the float32 rounding of the sums is as large.  (Two bf16 parts, as the other dense
 // layers have, issue at twice the rate and are good to 2^-17.)
 //
-// 573,894 slots of 286,947 rows, 32 experts: 256 -> 128 in 217 us (174 TFLOP/s), 128 -> 256 in 258 (146).  Neither memory (90 and 135 us)
+// 573,894 slots of 286,947 rows, 32 experts: 256 -> 128 in 230 us (163 TFLOP/s), 128 -> 256 in 268 (140).  Neither memory (90 and 135 us)
 // nor the tensor cores (115 us at their tf32 rate) set that: an instruction takes the warp that issues it some 50 cycles, twelve a chunk,
 // and a column block's accumulators are read out before the next block may use them.  One accumulator for both kinds of products, two of
 // them in turn, took 180 and 186 us and lost 1.1e-6 / 1.8e-6 of the result's norm with 128 / 256 terms where this loses 4e-7 / 9e-7; two
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(256) k_experts_split(int n_out, int n_in, int6
 // warps, rounded to nearest; after EG_FOLD such sums, 4,096 rows, these go to their place in memory and start again, so that no chain of
 // additions grows with the number of rows but that of the 4,096s (the bias gradient's are added in 64 bits).
 //
-// 573,894 slots, 256 -> 128, 32 experts: 297 us (127 TFLOP/s).  The column warps bound it, some 2,000 cycles a chunk of their own
+// 573,894 slots, 256 -> 128, 32 experts: 315 us (119 TFLOP/s).  The column warps bound it, some 2,000 cycles a chunk of their own
 // instructions where its products take 768; sixteen of them do not fit the registers beside the epilogue's sums.
 //
 // Roles: warp 0 issues the products, warps 2 - 5 hold dy's columns, 6 - 9 x's, 10 - 17 the sums (warp 1 has none).

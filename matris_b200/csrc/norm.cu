@@ -44,8 +44,8 @@ struct GnArgs {
   float* sums;             // backward: [n_seg, channels, 2]: sum dz, sum dz xh
 };
 
-// Blocks of a multiprocessor: three of the float32 forward pass (138 us at the size above; two 150, four 150), two of the others (the
-// backward pass 256 us, with three 274)
+// Blocks of a multiprocessor: three of the float32 forward pass, two of the others.  (573,894 float32 rows of 128 in 512 segments, eight
+// groups, when this was chosen: forward 138 us with three, 150 with two or four; backward 256 with two, 274 with three.  Now 131 and 235.)
 constexpr int gn_blocks(int v, bool forward = false) { return forward && v != 8 ? 3 : 2; }
 template <typename T, int V> struct Vec;
 template <> struct Vec<float, 4> { float4 r; };
@@ -175,7 +175,7 @@ template <int U, typename F> __device__ __forceinline__ void batches(int n, F f)
   if (left > 0) f(left, std::false_type{});
 }
 // The second pass reads and writes for the last time: both are marked so, which leaves L2 to the rows that the second pass is still to
-// find there (573,894 rows of 512 bytes by 512 segments: forward 148 -> 138 us, backward 301 -> 274).
+// find there (573,894 rows of 512 bytes in 512 segments: that step took the forward pass from 148 to 138 us, the backward one from 301 to 274).
 template <typename T, int V> struct Stream {
   const char* p;
   int64_t step;
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_group_norm_join(const __grid_con
           const int64_t c = c0 + 32 * i, f = max(from, c * a.chunk), t = min(to, (c + 1) * a.chunk);
           if (f >= t) break;
           const float nb = (float)(t - f);
-          join(n, mean, m2, nb, v[i].x, v[i].y / (float)cg);  // in units of rows: counts stay exact
+          join(n, mean, m2, nb, v[i].x, v[i].y / (float)cg);  // in units of rows: counts are exact up to 2^24, good to 2^-24 above
           n += nb;
         }
       }
@@ -854,7 +854,11 @@ static int gn_chunk(int64_t n_rows, int n_sm) {
   return (int)(r < 32 ? 32 : (r + 7) / 8 * 8);
 }
 // Longest segment that a block takes (slab by slab), -1: none.  Few rows: all of them, three launches fewer.  Segments that are long on
-// average: none.
+// average: none.  Forward, float32 rows of 128 in eight groups, even segments, by blocks / by chunks:
+//     1,024 rows of one segment 14.3 / 14.3 us, of eight 8.2 / 13.8;      2,048 rows of one 20.5 / 13.8;     8,192 of eight 14.3 / 16.4
+//     16,384 rows of four segments 32.8 / 20.5, of eight 22.5 / 19.9, of sixteen 14.4 / 20.5
+//     573,894 rows of 128 segments 166 / 160, of 280 135 / 160, of 512 123 / 160 (131 as it is: launches that find no long segment)
+// The line goes by the average: one long segment among short ones is left to a few blocks (15,000 of 16,000 rows 96 us, by chunks 23).
 static int gn_limit(int64_t n_rows, int n_seg) {
   if (n_rows <= 1024) return 1024;
   if (n_rows > 2048 * (int64_t)n_seg) return -1;

@@ -567,7 +567,8 @@ static int route_blocks(int64_t n_rows, int n_sm) {
   const int64_t most = 4 * (int64_t)n_sm, want = (n_rows + 63) / 64;
   return (int)(want < most ? (want > 0 ? want : 1) : most);
 }
-// few rows: one block does everything
+// Few rows: one block does everything.  (One block / three launches: 512 rows of 8 experts 10.2 / 12.3 us, 1,024 14.3 / 12.3, 2,048 22 / 12.3;
+// 64 rows of 64, top 6 11.8 / 16.4, 256 26.6 / 16.4; 16 rows of 256, top 8 12.3 / 22, 64 33 / 43.)
 static bool route_small(int64_t n_rows, int n_experts) { return n_rows * n_experts <= 4096; }
 static bool route_valid(const mb_route* d) {
   return d && d->n_rows >= 0 && d->n_experts >= 1 && d->n_experts <= RT_MAX_EXPERTS && d->top_k >= 1 && d->top_k <= RT_MAX_K &&
