@@ -55,3 +55,33 @@ def test_splits_that_make_room_stay_until_other_streams_have_read_them(ops):
     torch.cuda.synchronize()
     report("read late", y, product(x, w), 1e-4, scaled=True)
     assert len(over) == 400
+
+
+def test_threads_on_their_own_streams_share_plain_weights(ops):
+    """Four threads, each on a stream of its own, 300 weights between them: more than are kept, so that entries go while others read."""
+    import threading
+    weights = [torch.randn(128, 128, device="cuda") for _ in range(300)]
+    x = torch.randn(256, 128, device="cuda")
+    want = [product(x, w) for w in weights]
+    torch.cuda.synchronize()
+    errors, worst = [], [0.0] * 4
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for k in range(600):
+                    j = (k * (2 * i + 1) + 75 * i) % 300
+                    y = ops.linear(x, weights[j])
+                    worst[i] = max(worst[i], float((y.double() - want[j]).abs().max()))
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors[:3]
+    # 128 terms of size 1, operands of two bfloat16 parts: 2^-17 of each term
+    assert max(worst) <= 2.0 ** -17 * 128 * 4, worst
