@@ -561,6 +561,32 @@ def _here(*tensors):
     return device
 
 
+def _share(a, b):
+    """Whether two [rows, width] tensors with neighbouring values have memory in common."""
+    if not a.numel() or not b.numel():
+        return False
+    size, ends = a.element_size(), []
+    for t in (a, b):
+        first, (rows, width) = t.data_ptr(), t.shape
+        ends.append((first, first + ((rows - 1) * t.stride(0) + width) * size))
+    if ends[0][1] <= ends[1][0] or ends[1][1] <= ends[0][0]:
+        return False
+    lds = {t.stride(0) for t in (a, b) if t.shape[0] > 1}
+    if b.element_size() != size or len(lds) != 1 or (ends[1][0] - ends[0][0]) % size:
+        return True
+    ld = lds.pop()
+    at = (ends[1][0] - ends[0][0]) // size % ld  # columns of one wider tensor: b begins `at` columns behind a
+    return at < a.shape[1] or at + b.shape[1] > ld
+
+
+def _apart(out, name, t, may_be=False):
+    """``out`` and an input that the kernels read while they write: no memory in common (``may_be``: or the very same rows)."""
+    if t is None or (may_be and out.data_ptr() == t.data_ptr() and out.stride() == t.stride()):
+        return
+    if _share(out, t):
+        raise ValueError(f"out overlaps {name}")
+
+
 def _launch(name, struct_type, data, device):
     d = struct_type.from_buffer_copy(data)
     call(name, C.byref(d), _stream() if _raw_stream is None else _raw_stream(device))
@@ -603,13 +629,20 @@ def _norm_rows(x, weight, bias, seg_ptr, n_groups, act, eps):
     return x, rows, channels, ld, n_seg
 
 
-def _norm_out(like, rows, channels, out, seg_ptr):
+def _norm_out(like, rows, channels, out, seg_ptr, dy=None):
     """The output, its row stride, and whether rows of no segment are to be cleared."""
     if out is None:
         return torch.empty(like.shape, dtype=like.dtype, device=like.device), channels, 1
     if seg_ptr is None:
-        return _take(out, "out", like.dtype, like.shape), channels, 0
-    return out, _take_rows(out, "out", like.dtype, rows, channels), 0
+        _take(out, "out", like.dtype, like.shape)
+        ld = channels
+    else:
+        ld = _take_rows(out, "out", like.dtype, rows, channels)
+    flat = (rows, channels)
+    for name, t in (("x", like), ("dy", dy)):
+        if t is not None:
+            _apart(out if seg_ptr is not None else out.view(flat), name, t if seg_ptr is not None else t.view(flat), may_be=True)
+    return out, ld, 0
 
 
 def group_norm_fwd(x, weight, bias, n_groups, seg_ptr=None, eps=1e-5, act=0, out=None):
@@ -618,7 +651,8 @@ def group_norm_fwd(x, weight, bias, n_groups, seg_ptr=None, eps=1e-5, act=0, out
 
     ``x`` [rows, channels] with ``seg_ptr`` (int32 [segments + 1] row offsets on the device, as ``BatchedGraph.atom_ptr``), or
     [batch, .., channels] without.  Returns (y, stats): stats [segments, groups, 2] (mean, 1 / deviation) is what
-    ``group_norm_bwd`` reads.  Rows of no segment are zero in a returned tensor and left alone in a given ``out``, which may be x."""
+    ``group_norm_bwd`` reads.  Rows of no segment are zero in a returned tensor and left alone in a given ``out``, which may be x and does
+    not overlap it otherwise."""
     xr, rows, channels, ld, n_seg = _norm_rows(x, weight, bias, seg_ptr, n_groups, act, eps)
     device = _here(x, weight, bias, seg_ptr, out)
     y, ld_y, zero = _norm_out(x, rows, channels, out, seg_ptr)
@@ -645,7 +679,7 @@ def group_norm_bwd(dy, x, weight, bias, stats, n_groups, seg_ptr=None, act=0, ou
         ld_dy = _take_rows(dy, "dy", x.dtype, rows, channels)
     _take(stats, "stats", _F32, (n_seg, n_groups, 2))
     device = _here(x, dy, weight, bias, stats, seg_ptr, out)
-    dx, ld_dx, zero = _norm_out(x, rows, channels, out, seg_ptr)
+    dx, ld_dx, zero = _norm_out(x, rows, channels, out, seg_ptr, dy)
     if zero and not n_seg:
         dx.zero_()
     dweight = dbias = None
@@ -794,7 +828,7 @@ def experts_linear(x, weights, offsets, bias=None, idx=None, in_act=0, out_act=0
     of its transpose, the data gradient.  ``in_act`` / ``out_act`` 1: SiLU.  ``offsets``, ``idx``: ``Route.offsets``, ``Route.row_of``.
     Infinities in one operand and NaN give what they give in float32; infinite times infinite or subnormal values give NaN.
     A part of a grouping's offsets with the weights of those experts is a share of the work.  Slots of no expert, ahead of ``offsets[0]`` and
-    from ``offsets[-1]`` on, are zero in a returned tensor and left alone in a given ``out``, which must not overlap the inputs."""
+    from ``offsets[-1]`` on, are zero in a returned tensor and left alone in a given ``out``, which does not overlap x or ``gate``."""
     if not isinstance(weights, ExpertWeights):
         weights = ExpertWeights(weights)
     n_experts, n_out, n_in = weights.shape
@@ -812,7 +846,11 @@ def experts_linear(x, weights, offsets, bias=None, idx=None, in_act=0, out_act=0
         if bias.data_ptr() % 16:
             raise ValueError("bias has to start on a 16-byte boundary")
     ld_gate = 0 if gate is None else _take_rows(gate, "gate", _F32, n_slots, n_out, aligned=True)
-    ld_y = n_out if out is None else _take_rows(out, "out", _F32, n_slots, n_out, aligned=True)
+    ld_y = n_out
+    if out is not None:
+        ld_y = _take_rows(out, "out", _F32, n_slots, n_out, aligned=True)
+        _apart(out, "x", x)
+        _apart(out, "gate", gate)
     device = _here(x, weights.parts, offsets, bias, idx, gate, out)
     y = torch.empty((n_slots, n_out), dtype=_F32, device=x.device) if out is None else out
     _launch("mb_experts_linear", _lib.MbExperts, _EXPERTS_FMT.pack(
